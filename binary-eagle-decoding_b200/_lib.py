@@ -29,6 +29,9 @@ FLAG_SIGN_CHANGE = 128
 FLAG_TIMEOUT = 256
 FLAG_NONFINITE_FEATURES = 512
 FLAG_NONFINITE_LOSS = 1024
+FLAG_BAD_LENGTH = 2048
+FLAG_NO_PAGES = 4096
+FLAG_BAD_PAGE = 8192
 
 # Messages of the reference's ValueErrors for the same conditions.
 FLAG_MESSAGES = (
@@ -42,6 +45,9 @@ FLAG_MESSAGES = (
     (FLAG_SIGN_CHANGE, "bounded latent scale changed a sign"),
     (FLAG_NONFINITE_FEATURES, "nonfinite teacher features"),
     (FLAG_NONFINITE_LOSS, "nonfinite loss"),
+    (FLAG_BAD_LENGTH, "request lengths, page counts or row offsets out of range"),
+    (FLAG_NO_PAGES, "out of free cache pages"),
+    (FLAG_BAD_PAGE, "cache page or slot outside the pool"),
 )
 # Device-side failures that are not the reference's ValueErrors.
 FLAG_ERRORS = ((FLAG_TIMEOUT, "a bounded device wait timed out"),)
@@ -70,6 +76,17 @@ class FfnLargeArgs(ctypes.Structure):
         ("x", P), ("y", P), ("tokens", c_int64), ("hidden", c_int64), ("inter", c_int64),
         ("signs_gate_up_i8", P), ("scale_gate", P), ("scale_up", P), ("signs_down_i8", P), ("scale_down", P),
         ("hidden_out", P), ("workspace", P), ("workspace_bytes", c_size_t), ("flags", P),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", P), ("q_row", c_int64), ("q_head", c_int64), ("row_type", c_int), ("k_cache", P), ("v_cache", P),
+        ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3), ("cache_type", c_int), ("page_size", c_int),
+        ("pool_pages", c_int64), ("table", P), ("table_ld", c_int64), ("table_width", c_int), ("context", P),
+        ("starts", P), ("requests", c_int), ("rows", c_int64), ("heads", c_int), ("kv_heads", c_int),
+        ("head_dim", c_int), ("causal", c_int), ("window", c_int64), ("longest", c_int), ("scale", ctypes.c_float),
+        ("out", P), ("zero_fill", c_int), ("workspace", P), ("workspace_bytes", c_size_t), ("flags", P),
     ]
 
 
@@ -180,6 +197,12 @@ SIGNATURES = {
                             P, c_int64, P, P, c_int64, P, P]),
     "bd_context_kv_post": (c_int, [P, c_int, c_int64, c_int, c_int64, c_int, c_int, P, ctypes.c_float, ctypes.c_float,
                                    c_int64, P, P, c_int64, c_int64, P, P]),
+    "bd_page_plan": (c_int, [P, P, c_int, c_int, c_int64, P, c_int64, c_int, P, P, P, c_int64, P, P, P, P, P, c_int64,
+                             P, P]),
+    "bd_paged_store": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, P, c_int64, c_int, c_int, c_int,
+                               c_int64, P, P, P, P, c_int, P, P]),
+    "bd_paged_attention_workspace_bytes": (c_size_t, [c_int]),
+    "bd_paged_attention": (c_int, [ctypes.POINTER(PagedAttentionArgs), P]),
     "bd_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "bd_attention_decode": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, P,
                                     P, c_size_t, P]),
@@ -216,7 +239,7 @@ def load() -> ctypes.CDLL:
 
 # Kernel launches issued by each entry point (for launch accounting).
 KERNELS_PER_CALL = {"bd_ffn_he4": 3, "bd_ffn_he4_fused": 2, "bd_loss_head_forward": 3, "bd_ffn_w1": 4, "bd_attention_decode": 2, "bd_attention_decode_x16": 2,
-                    "bd_accept_rejection": 2,
+                    "bd_accept_rejection": 2, "bd_paged_attention": 2,
                     "bd_ste_grad_prep": 2, "bd_ste_input_backward": 2, "bd_train_attention_backward": 3}
 launches = 0
 

@@ -8,7 +8,9 @@ caller, for deferred checks) reads them.
 
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -586,4 +588,194 @@ def argmax_rows(logits: Tensor, flags: Flags | None = None) -> Tensor:
     _lib.call("bd_argmax_rows_bf16", _p(logits), rows, logits.shape[-1], _p(out), flags.ptr, _stream(device))
     if own:
         flags.check()
+    return out
+
+
+# --------------------------------------------------------------------------- paged cache
+
+_ROW_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_ATTENDS = {(torch.float32, torch.float16), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)}
+PAGE_SIZES = (8, 16, 32, 64, 128, 256)
+
+
+class PagePlan(NamedTuple):
+    """Rows of one step: request ``b`` has rows ``starts[b] .. starts[b + 1]``, each at
+    ``positions[row]`` of its request and at ``slots[row]`` of the cache."""
+
+    starts: Tensor
+    positions: Tensor
+    slots: Tensor
+
+
+def _same_device(*tensors: Tensor) -> torch.device:
+    device = tensors[0].device
+    if device.type != "cuda":
+        raise ValueError("bitdraft kernels take CUDA tensors")
+    for t in tensors:
+        if t.device != device:
+            raise ValueError("all tensors must be on one device")
+    return device
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for a launch (its streams and kernels belong to it)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _int32(name: str, t: Tensor, *shape: int) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)}")
+
+
+def _check_table(table: Tensor, requests: int) -> None:
+    if table.dtype != torch.int32 or table.ndim != 2 or table.shape[0] != requests or table.shape[1] < 1 \
+            or (table.shape[1] > 1 and table.stride(1) != 1) or (requests > 1 and table.stride(0) < table.shape[1]):
+        raise ValueError("table must be int32 [requests, pages of a request] with unit column stride")
+
+
+def _table_ld(table: Tensor) -> int:
+    return max(table.stride(0), table.shape[1])
+
+
+def _check_caches(k_cache: Tensor, v_cache: Tensor) -> None:
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype \
+            or k_cache.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("caches must be fp16 or bf16 [pages, page_size, kv_heads, head_dim], both alike")
+    if k_cache.shape[0] < 1 or k_cache.shape[1] not in PAGE_SIZES:
+        raise ValueError("page_size must be a power of two from 8 to 256, in at least one page")
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("caches need unit stride within a head")
+
+
+def _strides(cache: Tensor):
+    return (_lib.c_int64 * 3)(*cache.stride()[:3])
+
+
+def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free: Tensor, top: Tensor, page_size: int,
+              rows: int, pool_pages: int, owned_out: Tensor | None = None, top_out: Tensor | None = None,
+              flags: Flags | None = None) -> PagePlan:
+    """Pages and rows of one step of a paged cache, from lengths on the device.
+
+    ``context`` and ``count`` int32 ``[B]`` are the cached positions and new tokens of
+    each request, ``table`` int32 ``[B, P]`` its pages in order of position, ``owned``
+    int32 ``[B]`` how many it has, ``free`` int32 a stack of free pages of which
+    ``top`` int32 ``[1]`` are left.  Every request then owns exactly the pages that
+    ``context + count`` positions need: missing ones are taken from the stack, those
+    beyond are given back (a finished request has both lengths 0).  ``table`` and
+    ``free`` change in place, ``owned`` and ``top`` too unless ``owned_out`` and
+    ``top_out`` are given.  Returns ``starts [B + 1]`` and, for ``rows`` rows,
+    ``positions`` and ``slots`` (-1 behind the last request).  Without ``flags`` the
+    call waits and raises ``ValueError`` for lengths that do not fit or a lack of pages."""
+    requests = context.shape[0] if context.ndim == 1 else 0
+    if requests < 1:
+        raise ValueError("a plan needs int32 lengths of at least one request")
+    _int32("context", context, requests)
+    _int32("count", count, requests)
+    _int32("owned", owned, requests)
+    _int32("top", top, 1)
+    _int32("free", free, free.numel())
+    owned_out = owned if owned_out is None else owned_out
+    top_out = top if top_out is None else top_out
+    _int32("owned_out", owned_out, requests)
+    _int32("top_out", top_out, 1)
+    _check_table(table, requests)
+    if page_size not in PAGE_SIZES:
+        raise ValueError("page_size must be a power of two from 8 to 256")
+    if rows < 0:
+        raise ValueError("rows must not be negative")
+    device = _same_device(context, count, table, owned, free, top, owned_out, top_out)
+    with _on(device):
+        out = torch.empty(requests + 1 + 2 * rows, dtype=torch.int32, device=device)
+        starts, positions, slots = out[:requests + 1], out[requests + 1:requests + 1 + rows], out[requests + 1 + rows:]
+        own = flags is None
+        flags = flags or Flags(device)
+        _lib.call("bd_page_plan", _p(context), _p(count), requests, page_size, pool_pages, _p(table), _table_ld(table),
+                  table.shape[1], _p(owned), _p(owned_out), _p(free), free.numel(), _p(top), _p(top_out), _p(starts),
+                  _p(positions), _p(slots), rows, flags.ptr, _stream(device), kernels=1 + (rows > _PLAN_ROWS))
+        if own:
+            flags.check()
+    return PagePlan(starts, positions, slots)
+
+
+_PLAN_ROWS = 4096  # rows that the plan's one CTA fills itself
+
+
+def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor, flags: Flags | None = None) -> None:
+    """Key and value rows ``[rows, kv_heads, head_dim]`` (fp32, fp16 or bf16; views of a
+    fused projection are fine) into slots ``page * page_size + offset`` of the caches
+    ``[pages, page_size, kv_heads, head_dim]``, rounded to their type.  Rows with slot -1 are
+    skipped; a slot may appear once.  Raises (or flags) "F16 cache storage overflow"
+    when a stored value is not finite."""
+    _check_caches(k_cache, v_cache)
+    rows = k.shape[0] if k.ndim == 3 else -1
+    if rows < 0 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ROW_TYPE or k.shape[1:] != k_cache.shape[2:]:
+        raise ValueError("k and v must be fp32, fp16 or bf16 [rows, kv_heads, head_dim] of the caches' heads")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("k and v need unit stride within a head")
+    _int32("slots", slots, rows)
+    device = _same_device(k, v, slots, k_cache, v_cache)
+    with _on(device):
+        own = flags is None
+        flags = flags or Flags(device)
+        pages, page_size, kv_heads, head_dim = k_cache.shape
+        _lib.call("bd_paged_store", _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _ROW_TYPE[k.dtype],
+                  _p(slots), rows, kv_heads, head_dim, page_size, pages, _p(k_cache), _strides(k_cache), _p(v_cache),
+                  _strides(v_cache), _ROW_TYPE[k_cache.dtype], flags.ptr, _stream(device))
+        if own:
+            flags.check()
+
+
+def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, context: Tensor, starts: Tensor,
+                    causal: bool = True, window: int | None = None, scale: float | None = None,
+                    longest: int | None = None, out: Tensor | None = None, flags: Flags | None = None) -> Tensor:
+    """Attention of every request's new tokens over its keys in a paged cache.
+
+    ``q [rows, heads, head_dim]``: request ``b`` has rows ``starts[b] .. starts[b + 1]`` at
+    positions ``context[b] ..``; their own keys and values are in the cache already
+    (``paged_store``).  A token sees the request's keys at or before its position, or all
+    of them when not ``causal`` (a draft block), and with ``window`` only those less
+    than ``window`` positions away.  fp32 rows over an fp16 cache (the products keep
+    fp32 precision), fp16 over fp16 or bf16 over bf16; head_dim 64 or 128.
+    ``longest``: an upper bound of the requests' new tokens, when the caller knows
+    one.  Returns ``out``, whose rows of no request stay as they were; without ``out``
+    a new tensor in which they are zero."""
+    _check_caches(k_cache, v_cache)
+    if q.ndim != 3 or (q.dtype, k_cache.dtype) not in _ATTENDS:
+        raise ValueError("q must be [rows, heads, head_dim]: fp32 or fp16 over fp16 caches, bf16 over bf16")
+    rows, heads, head_dim = q.shape
+    pages, page_size, kv_heads, cache_dim = k_cache.shape
+    if head_dim != cache_dim or head_dim not in (64, 128) or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError("head_dim must be 64 or 128, the caches' own, and heads a multiple of kv_heads")
+    if q.stride(2) != 1:
+        raise ValueError("q needs unit stride within a head")
+    requests = context.shape[0] if context.ndim == 1 else 0
+    _int32("context", context, requests)
+    _int32("starts", starts, requests + 1)
+    _check_table(table, requests)
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1")
+    if longest is not None and longest < 1:
+        raise ValueError("longest must be at least 1")
+    device = _same_device(q, k_cache, v_cache, table, context, starts)
+    fresh = out is None
+    if not fresh and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
+        raise ValueError("out must be contiguous and like q")
+    with _on(device):
+        if fresh:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        nbytes = _lib.size("bd_paged_attention_workspace_bytes", head_dim)
+        # a buffer of this call: concurrent streams and captured graphs share none
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        own = flags is None
+        flags = flags or Flags(device)
+        args = _lib.PagedAttentionArgs(
+            _p(q), q.stride(0), q.stride(1), _ROW_TYPE[q.dtype], _p(k_cache), _p(v_cache), k_cache.stride()[:3],
+            v_cache.stride()[:3], _ROW_TYPE[k_cache.dtype], page_size, pages, _p(table), _table_ld(table),
+            table.shape[1], _p(context), _p(starts), requests, rows, heads, kv_heads, head_dim, int(causal),
+            window or 0, min(longest or 0, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, _p(out),
+            int(fresh), _p(ws), nbytes, flags.ptr,
+        )
+        _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device))
+        if own:
+            flags.check()
     return out

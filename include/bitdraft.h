@@ -47,6 +47,9 @@ typedef struct CUstream_st *bd_stream_t; /* == cudaStream_t */
 #define BD_FLAG_TIMEOUT 256u          /* a bounded device wait ran out (the kernel returned early) */
 #define BD_FLAG_NONFINITE_FEATURES 512u /* captures.py:129-130 "nonfinite teacher features" */
 #define BD_FLAG_NONFINITE_LOSS 1024u    /* worker.py:360-361 "nonfinite loss" */
+#define BD_FLAG_BAD_LENGTH 2048u        /* a request's length, page count or row offset does not fit */
+#define BD_FLAG_NO_PAGES 4096u          /* the free pages do not cover a request's new tokens */
+#define BD_FLAG_BAD_PAGE 8192u          /* a needed page id or slot is outside the cache */
 
 int bd_abi_version(void);
 const char *bd_status_string(int status);
@@ -420,6 +423,93 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
                         int kv_heads, int head_dim, int keys, int windowed, int64_t anchor, int64_t window,
                         int64_t stable_keys, float *out, void *workspace, size_t workspace_bytes,
                         bd_stream_t stream);
+
+/* ==================================================================== paged cache
+ * A key/value cache shared by requests of different lengths: rows live in pages
+ * [pages][page_size][kv_heads][head_dim] (element strides given, the last 1), and
+ * table[b][j] is the page of positions j page_size .. of request b.  The reference
+ * serves one request per process and keeps no cache (model.py:382-396 recomputes
+ * the context); its runtime's cache is not vendored.  All lengths are read on the
+ * device, so a captured graph replays with new ones.  page_size is a power of two
+ * from 8 to 256; positions and slots are 32-bit.
+ *
+ * bd_page_plan: one step's pages and rows from the lengths.  With need_b =
+ * ceil((context[b] + count[b]) / page_size), a request that owns more pages gives
+ * the last ones back (their entries become -1) and one that owns fewer takes the
+ * missing ones: with S = free_list[0 .. *top_in) followed by the pages given back
+ * in order of request and entry, the missing entries, in the same order, are
+ * S[|S| - 1], S[|S| - 2], ...  owned_out and top_out (which may be owned_in and
+ * top_in) receive the new counts.  A request whose missing pages do not all fit
+ * takes none (BD_FLAG_NO_PAGES).  starts[requests + 1]: exclusive sums of count;
+ * positions / slots of each of `rows` rows: context[b] + t and page x page_size +
+ * offset (slot -1 for a token without a page), -1 both behind the last request.
+ * A request with lengths below zero or beyond table_width pages keeps its pages
+ * and has no rows (BD_FLAG_BAD_LENGTH, as for more rows than `rows`, a top outside
+ * [0, free_capacity] and a full stack); page ids outside [0, pool_pages) are not
+ * used (BD_FLAG_BAD_PAGE).  Table entries of a request beyond the pages it owns are
+ * not read.
+ *
+ * bd_paged_store: key and value row r (row and head strides in elements; 16-byte
+ * aligned pieces) to slot slots[r] of the caches, rounded to their type; slots below
+ * 0 are skipped, slots beyond the cache too (BD_FLAG_BAD_PAGE).  A stored value
+ * that is not finite sets BD_FLAG_CACHE_OVERFLOW (model.py:100-101).  A slot given
+ * twice in one call holds pieces of either row.  Strides: host int64 [3] (page,
+ * slot, head), multiples of 8.
+ *
+ * bd_paged_attention: for token t of request b (row starts[b] + t, position
+ * context[b] + t), out = softmax_s(scale q . k_s) v_s over the cached keys s <
+ * context[b] + count (count = starts[b + 1] - starts[b]; the new tokens' own keys are
+ * stored first), s <= position when causal, |position - s| < window when window >
+ * 0.  Query head h reads kv head h / (heads / kv_heads).  head_dim 64 or 128.
+ * Types: fp32 rows over an fp16 cache at fp32 precision, fp16 over fp16, bf16 over
+ * bf16; out [rows][heads][head_dim] has the type of q.  longest: no request has
+ * more new tokens (0: unknown); it saves the launch of kernels that no request
+ * needs.  Rows of no request are left as they were, or set to zero when zero_fill.
+ * A request whose lengths do not fit (rows, table_width, longest) is left out
+ * (BD_FLAG_BAD_LENGTH); keys on a page outside the pool count as zeros
+ * (BD_FLAG_BAD_PAGE); entries of pages that no token sees are not read.  What the
+ * cache holds at keys that a row does not see never reaches it, not even as NaN.
+ * The workspace needs no clearing; calls that overlap on the GPU need their own. */
+#define BD_F16 0
+#define BD_BF16 1
+#define BD_F32 2
+int bd_page_plan(const int32_t *context, const int32_t *count, int requests, int page_size, int64_t pool_pages,
+                 int32_t *table, int64_t table_ld, int table_width, const int32_t *owned_in, int32_t *owned_out,
+                 int32_t *free_list, int64_t free_capacity, const int32_t *top_in, int32_t *top_out, int32_t *starts,
+                 int32_t *positions, int32_t *slots, int64_t rows, int32_t *flags, bd_stream_t stream);
+int bd_paged_store(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                   int row_type, const int32_t *slots, int64_t rows, int kv_heads, int head_dim, int page_size,
+                   int64_t pool_pages, void *k_cache, const int64_t *k_strides, void *v_cache,
+                   const int64_t *v_strides, int cache_type, int32_t *flags, bd_stream_t stream);
+typedef struct {
+    const void *q;
+    int64_t q_row, q_head; /* strides in elements */
+    int row_type;
+    const void *k_cache, *v_cache;
+    int64_t k_strides[3], v_strides[3]; /* page, slot, head */
+    int cache_type;
+    int page_size;
+    int64_t pool_pages;
+    const int32_t *table; /* [requests][table_ld] */
+    int64_t table_ld;
+    int table_width;
+    const int32_t *context; /* [requests] */
+    const int32_t *starts;  /* [requests + 1] */
+    int requests;
+    int64_t rows;
+    int heads, kv_heads, head_dim;
+    int causal;
+    int64_t window;
+    int longest;
+    float scale;
+    void *out;
+    int zero_fill;
+    void *workspace; /* 16-byte aligned */
+    size_t workspace_bytes;
+    int32_t *flags;
+} bd_paged_attention_args;
+size_t bd_paged_attention_workspace_bytes(int head_dim);
+int bd_paged_attention(const bd_paged_attention_args *args, bd_stream_t stream);
 
 /* ================================================================ row-wise chains (training)
  * bd_rms_forward: out = x * rsqrt(mean(x^2) + eps) * w over rows of cols
