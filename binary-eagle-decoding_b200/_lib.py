@@ -239,7 +239,7 @@ def load() -> ctypes.CDLL:
 
 # Kernel launches issued by each entry point (for launch accounting).
 KERNELS_PER_CALL = {"bd_ffn_he4": 3, "bd_ffn_he4_fused": 2, "bd_loss_head_forward": 3, "bd_ffn_w1": 4, "bd_attention_decode": 2, "bd_attention_decode_x16": 2,
-                    "bd_accept_rejection": 2, "bd_paged_attention": 2,
+                    "bd_accept_rejection": 2,
                     "bd_ste_grad_prep": 2, "bd_ste_input_backward": 2, "bd_train_attention_backward": 3}
 launches = 0
 

@@ -1,6 +1,8 @@
 // Work split and row helpers of the paged attention, shared by its kernels.
 #pragma once
 
+#include <cuda.h>
+
 #include "paged.cuh"
 
 namespace bd {
@@ -10,6 +12,8 @@ enum PagedMode : int {
     PAGED_F16 = 1,   // fp16 rows and cache
     PAGED_BF16 = 2,  // bf16 rows and cache
 };
+
+struct PagedOpen;
 
 struct PagedArgs {
     const void *q;
@@ -29,7 +33,12 @@ struct PagedArgs {
     void *out;
     int64_t out_row;  // heads stand head_dim apart
     int zero_fill;
-    float *part_o, *part_ml;  // [2 x CTAs][rows of an item][head_dim], [..][2]
+    int split_rows;  // requests of more rows per kv head go to the tcgen05 kernel (INT_MAX: none)
+    // partials of the two kernels: [2 x CTAs][rows of an item][head_dim] and [..][2], and what to join
+    struct Parts {
+        float *o, *ml;
+        PagedOpen *open;  // [CTAs]
+    } parts[2];
     int32_t *flags;
 };
 
@@ -103,30 +112,40 @@ __device__ __forceinline__ int64_t paged_row_offset(const PagedArgs &a, const Pa
            (static_cast<int64_t>(it.h) * a.groups + (row - t * a.groups)) * head_stride;
 }
 
+// An item that a CTA begins and does not end: its partials are place 2 c + 1 of this
+// CTA c and places 2 d of the CTAs d = c + 1 .. last.
+struct PagedOpen {
+    PagedItem it;
+    int last;  // -1: no such item
+};
+
 struct PagedShared {
     int64_t warp_sums[32];
     int64_t before;
     int b;
 };
 
-// The walk over the units of this CTA's range, see the head of paged_attention.cu.
-// M rows to an item, KT keys to a unit.  Requests of more than `above` rows (0: all)
-// are walked, or of at most `upto` rows.
-template <int M, int KT>
+// The walk over the units of this CTA's range, see the head of paged_attention.cu: the
+// items of M rows and units of KT keys of the requests of one kernel (TC: those of
+// more than a.split_rows rows per kv head, else the others).
+template <int M, int KT, bool TC>
 struct PagedWalk {
-    int64_t u, end, total, per;
-    int cta, off;          // off: units of the current item before u
+    int cta, at, len, per;      // this CTA's range: units done, in all, and of every CTA's range but the last
+    int off;                    // units of the current item before the range
     int b, h, i, tiles, units;  // units: of the item
     PagedRequest r;
-    PagedItem it;
 
     static __device__ __forceinline__ int item_units(const PagedItem &x) { return (x.hi + KT - 1) / KT - x.lo / KT; }
+    static __device__ __forceinline__ int request_tiles(const PagedArgs &a, const PagedRequest &r) {
+        const int rows = r.count * a.groups;
+        return (rows > a.split_rows) == TC ? (rows + M - 1) / M : 0;
+    }
 
     // Units of one kv head of request b.
     static __device__ __forceinline__ int64_t request_units(const PagedArgs &a, int b) {
         const PagedRequest r = paged_request(a, b);
         if (r.bad) set_flag(a.flags, BD_FLAG_BAD_LENGTH);
-        const int tiles = (r.count * a.groups + M - 1) / M;
+        const int tiles = request_tiles(a, r);
         int64_t sum = 0;
         for (int i = 0; i < tiles; ++i) {
             PagedItem x;
@@ -158,9 +177,9 @@ struct PagedWalk {
 
     __device__ __forceinline__ void set_request(const PagedArgs &a) {
         r = paged_request(a, b);
-        tiles = (r.count * a.groups + M - 1) / M;
+        tiles = request_tiles(a, r);
     }
-    __device__ __forceinline__ void set_item(const PagedArgs &a) {
+    __device__ __forceinline__ void set_item(const PagedArgs &a, PagedItem &it) {
         paged_item<M>(a, r, i, it);
         it.b = b;
         it.h = h;
@@ -171,21 +190,22 @@ struct PagedWalk {
     __device__ __forceinline__ bool begin(const PagedArgs &a, PagedShared &sh, int cta_, int ctas) {
         cta = cta_;
         const int n = blockDim.x, tid = threadIdx.x;
-        int64_t w = tid < a.requests ? request_units(a, tid) * a.kv_heads : 0, sum;
-        int64_t incl = scan(w, sh, sum);
-        total = sum;
+        int64_t w = tid < a.requests ? request_units(a, tid) * a.kv_heads : 0, total, sum;
+        int64_t incl = scan(w, sh, total);
         for (int b0 = n; b0 < a.requests; b0 += n) {
             scan(b0 + tid < a.requests ? request_units(a, b0 + tid) * a.kv_heads : 0, sh, sum);
             total += sum;
         }
-        per = (total + ctas - 1) / ctas;
-        u = cta * per;
-        end = min(u + per, total);
-        if (u >= end) return false;
+        per = static_cast<int>((total + ctas - 1) / ctas);
+        const int64_t u = static_cast<int64_t>(cta) * per;
+        if (u >= total) return false;
+        at = 0;
+        len = static_cast<int>(min(static_cast<int64_t>(per), total - u));
         // the request that holds unit u
         int64_t before = 0;
+        sum = total;
         for (int b0 = 0; b0 < a.requests; b0 += n) {
-            if (b0 > 0 || a.requests > n) {
+            if (a.requests > n) {
                 w = b0 + tid < a.requests ? request_units(a, b0 + tid) * a.kv_heads : 0;
                 incl = scan(w, sh, sum);
             }
@@ -202,6 +222,7 @@ struct PagedWalk {
         set_request(a);
         // its kv head and rows
         int64_t each = 0;
+        PagedItem it;
         for (int j = 0; j < tiles; ++j) {
             paged_item<M>(a, r, j, it);
             each += item_units(it);
@@ -209,7 +230,7 @@ struct PagedWalk {
         h = static_cast<int>(rest / each);
         rest -= h * each;
         for (i = 0;; ++i) {
-            set_item(a);
+            set_item(a, it);
             if (rest < units) break;
             rest -= units;
         }
@@ -217,17 +238,18 @@ struct PagedWalk {
         return true;
     }
 
-    __device__ __forceinline__ bool more() const { return u < end; }
+    __device__ __forceinline__ bool more() const { return at < len; }
 
-    // The next stay: an item, its key tiles [kt0, kt1), and the partial it leaves (-1: it is done whole).
-    __device__ __forceinline__ void take(const PagedArgs &a, PagedItem &item, int &kt0, int &kt1, int &part) {
-        item = it;
-        const int n = static_cast<int>(min(static_cast<int64_t>(units - off), end - u));
+    // The next stay: an item, its key tiles [kt0, kt1), and the place of the partial it
+    // leaves (-1: it is done whole).  An odd place is an item that later CTAs end.
+    __device__ __forceinline__ void take(const PagedArgs &a, PagedItem &it, int &kt0, int &kt1, int &part) {
+        set_item(a, it);
+        const int n = min(units - off, len - at);
         kt0 = it.lo / KT + off;
         kt1 = kt0 + n;
         part = off == 0 && n == units ? -1 : 2 * cta + (off == 0);
-        u += n;
-        if (u >= end) return;
+        at += n;
+        if (at >= len) return;
         off = 0;
         if (++i == tiles) {
             i = 0;
@@ -239,28 +261,17 @@ struct PagedWalk {
                 } while (tiles == 0);
             }
         }
-        set_item(a);
     }
 
-    // The item around the border before range c, if that border is the first one inside it;
-    // its partials are those of CTAs first .. last.
-    __device__ __forceinline__ bool border(const PagedArgs &a, PagedShared &sh, int c, int ctas, PagedItem &item, int &first,
-                                           int &last) {
-        if (!begin(a, sh, c, ctas) || off == 0) return false;
-        const int64_t start = u - off;
-        if ((c - 1) * per > start) return false;
-        item = it;
-        first = c - 1;
-        last = static_cast<int>((start + units - 1) / per);
-        return true;
-    }
+    // The CTA that ends the item of the last stay, which began at its first unit with n units here.
+    __device__ __forceinline__ int last_cta(int n) const { return cta + (at - n + units - 1) / per; }
 };
 
 // One row by one warp, key by key: for rows whose tile products met values that are
 // not finite.  There a masked key's infinity or NaN times the zero of its weight
 // would reach the row, so only keys that the row sees are touched here.
 template <int D, int MODE>
-__device__ __noinline__ void paged_slow_row(const PagedArgs &a, const PagedItem &it, int row) {
+__device__ __forceinline__ void paged_slow_row(const PagedArgs &a, const PagedItem &it, int row) {
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31;
     __syncwarp();
@@ -326,5 +337,115 @@ __device__ __forceinline__ void paged_zero_rows(const PagedArgs &a) {
     for (int b = blockIdx.x; b < a.requests; b += gridDim.x)
         if (paged_request(a, b).bad) zero(clamp(a.starts[b]), clamp(a.starts[b + 1]), 1);
 }
+
+// ------------------------------------------------------------------ tiles
+//
+// Both attention kernels read K and V in tiles of 128 keys of one kv head, D / 64
+// blocks of 128 rows of 64 values (128 bytes, 128-byte-swizzled), which one warp
+// loads by TMA, a lane to a box of one page piece and block, into a ring of stages
+// that the other warps release.
+
+constexpr int kTileKeys = 128;
+constexpr int kRowsItem = 64;  // rows of an item: mma.sync kernel
+constexpr int kTcItem = 256;   // tcgen05 kernel
+constexpr int kMaxStages = 8;
+constexpr uint32_t kTilePolls = 1u << 21;
+
+template <int D>
+constexpr int tile_bytes() {
+    return kTileKeys * D * 2;
+}
+
+struct TileRing {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    volatile int abort;
+};
+
+// Waits for phase `count` (0, 1, ..) of a barrier.  A wait that runs out sets `abort`,
+// after which all waits pass: every role walks to its end.
+__device__ __forceinline__ void tile_wait(TileRing &ring, uint64_t *b, uint32_t count) {
+    for (uint32_t i = 0; i < kTilePolls; ++i)
+        if (mbar_try_wait(b, count & 1) || ring.abort) return;
+    ring.abort = 1;
+}
+__device__ __forceinline__ void tile_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+
+// The places in the ring of a stay's tiles, in order of use.  interleaved: keys and
+// values of a tile one after the other; else the keys run two tiles ahead.
+struct TileOrder {
+    bool interleaved;
+    int n;
+    __device__ __forceinline__ int key_at(int j) const { return interleaved ? 2 * j : (j < 2 ? j : 2 * j - 1); }
+    __device__ __forceinline__ int value_at(int j) const {
+        if (interleaved) return 2 * j + 1;
+        return n == 1 ? 1 : (j + 2 < n ? 2 * j + 2 : j + n);
+    }
+};
+
+struct PagedMaps {
+    CUtensorMap k, v;
+    int heads_outer;  // coordinates (column, slot, head, page), else (column, head, slot, page)
+};
+
+// The loading warp's whole run.  A piece without a key that some row sees, or on a page
+// outside the pool, is read as zeros (a box behind the last page).
+template <int D, int STAGES, typename Walk>
+__device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileRing &ring, uint8_t *stages,
+                                           const CUtensorMap *k_map, const CUtensorMap *v_map, int heads_outer,
+                                           int alternating_rows) {
+    const int lane = threadIdx.x & 31;
+    asm volatile("fence.proxy.async.global;" ::: "memory");  // the cache rows that earlier kernels wrote
+    const int piece = 1 << min(a.page_shift, 7);             // keys of a box
+    const int pieces = kTileKeys / piece;
+    const int block = lane / pieces, part = lane - block * pieces;
+    uint32_t place = 0;
+    while (walk.more()) {
+        PagedItem it;
+        int kt0, kt1, out;
+        walk.take(a, it, kt0, kt1, out);
+        const TileOrder order{it.r1 - it.r0 > alternating_rows, kt1 - kt0};
+        const int32_t *table = a.table + it.b * a.table_ld;
+        int next_key = 0, next_value = 0;
+        for (int i = 0; i < 2 * order.n; ++i, ++place) {
+            const bool value = next_key == order.n || order.value_at(next_value) == i;
+            const int kt = kt0 + (value ? next_value++ : next_key++);
+            const int key = kt * kTileKeys + part * piece;
+            const bool seen = block < D / 64 && key < it.hi && key + piece > it.lo;
+            int page = seen ? __ldg(table + (key >> a.page_shift)) : -1;
+            const uint32_t s = place % STAGES;
+            if (place >= STAGES) tile_wait(ring, &ring.empty[s], place / STAGES - 1);
+            if (ring.abort) continue;
+            if (lane == 0) mbar_expect_tx(&ring.full[s], tile_bytes<D>());
+            __syncwarp();
+            if (block < D / 64) {
+                if (page < 0 || page >= a.pool) {
+                    if (seen) set_flag(a.flags, BD_FLAG_BAD_PAGE);
+                    page = static_cast<int>(a.pool);
+                }
+                const int slot = key & ((1 << a.page_shift) - 1);
+                asm volatile(
+                    "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+                    "%5, %6}], [%2];" ::"r"(smem_u32(stages + s * tile_bytes<D>() + block * 16384 + part * piece * 128)),
+                    "l"(value ? v_map : k_map), "r"(smem_u32(&ring.full[s])), "r"(block * 64),
+                    "r"(heads_outer ? slot : it.h), "r"(heads_outer ? it.h : slot), "r"(page)
+                    : "memory");
+            }
+            __syncwarp();
+        }
+    }
+    // after a wait ran out: the copies in flight land before the CTA ends
+    if (ring.abort)
+        for (uint32_t j = place > STAGES ? place - STAGES : 0; j < place; ++j)
+            mbar_wait_bounded(&ring.full[j % STAGES], (j / STAGES) & 1, kTilePolls);
+}
+
+// ------------------------------------------------------------------ launches
+
+// Tensor maps of the caches; false when their strides cannot be expressed.
+bool paged_maps(const PagedArgs &a, int head_dim, bool bf16, PagedMaps &maps);
+int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream);
+int launch_paged_tc(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream);
 
 }  // namespace bd

@@ -1,0 +1,471 @@
+// Attention over the paged cache on the 5th-generation tensor cores (tcgen05, TMEM),
+// for fp16 and bf16 rows.  The mathematics, the item / unit / range split and the
+// joining of partials are those of paged_attention.cu, with 256 rows to an item and
+// 128 keys to a unit.
+//
+// One CTA per SM, 10 warps.  Two streams of work alternate on the tensor pipe so
+// that the softmax of one runs under the products of the other:
+//   * an item of more than 128 rows: stream t has rows [128 t, 128 t + 128), and both
+//     use every key tile, which is loaded once;
+//   * an item of up to 128 rows: both streams have the same rows, stream t takes every
+//     second key tile, and the two (maximum, sum, O) are joined at the end.
+// Warps 0-3 and 4-7 are the softmax of stream 0 and 1, a thread to a row: S from
+// TMEM, running maximum and sum, P as 16-bit values back over S's columns.  O stays
+// in TMEM; a row's O is rescaled only when its maximum has grown by more than 2^8
+// since the last time (P is at most 2^8 then, the sum and O scale alike), which
+// takes the rescaling off the usual path.  Warp 8 loads key and value tiles by TMA
+// (a box per page piece and 64 columns) into one ring in the order of their use;
+// warp 9 issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM,
+// V as it lies, its rows being the reduction).
+//
+// Every wait is bounded; one that runs out sets BD_FLAG_TIMEOUT and turns the waits
+// that follow into passes, so that all roles walk to their end.
+#include "paged_attention.cuh"
+
+namespace bd {
+
+constexpr int kTcThreads = 384;  // warps 10 and 11 only lend their registers
+constexpr float kTcSlack = 8.0f;  // growth of a maximum (log2) that leaves O as it is
+
+template <int D>
+constexpr int tc_stages() {
+    return D == 128 ? 5 : 8;
+}
+template <int D>
+constexpr size_t tc_smem() {
+    return 1024 + 2 * 128 * D * 2 + static_cast<size_t>(tc_stages<D>()) * tile_bytes<D>();
+}
+
+struct TcShared {
+    TileRing ring;
+    uint64_t q_full, s_full[2], p_full[2], o_full[2], drain;
+    uint32_t tmem;
+    float2 ml[128];
+    PagedShared walk;
+};
+
+__device__ __forceinline__ void tc_commit(uint64_t *b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 lanes x 32 columns of TMEM: lane = row, register = column.
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
+        "%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operands are 128-byte-swizzled rows of 64 values; a tile of D
+// columns is D / 64 such blocks of 128 rows (16 KB) one behind the other.
+// K-major (Q, K): 8-row groups 1024 B apart, a step of 16 columns is 32 B.
+__device__ __forceinline__ uint64_t tc_desc_rows(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// MN-major (V, whose rows are the reduction): 64-column blocks 16 KB apart, 8-row
+// groups 1024 B apart, a step of 16 rows is 2 KB.
+__device__ __forceinline__ uint64_t tc_desc_cols(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(16384 >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16 instruction descriptor: fp32 accumulators, M = 128, A and B fp16 or bf16.
+__host__ __device__ constexpr uint32_t tc_idesc(bool bf16, int n, bool b_cols) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_cols ? 1u : 0u) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    paged_tc_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                    int heads_outer) {
+    constexpr int MODE = BF16 ? PAGED_BF16 : PAGED_F16;
+    constexpr int kStages = tc_stages<D>(), kStage = tile_bytes<D>(), kBlocks = D / 64;
+    constexpr uint32_t kO = 256;  // TMEM columns: S0, S1 (P over them), O0, O1 at 256 and 384
+    extern __shared__ uint8_t tc_raw[];
+    uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *ring = sq + 2 * 128 * D * 2;
+    __shared__ TcShared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&sh.ring.full[s], 1);
+            mbar_init(&sh.ring.empty[s], 1);
+        }
+        mbar_init(&sh.q_full, 8);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sh.s_full[t], 1);
+            mbar_init(&sh.p_full[t], 4);
+            mbar_init(&sh.o_full[t], 1);
+        }
+        mbar_init(&sh.drain, 1);
+        sh.ring.abort = 0;
+        mbar_init_fence();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    grid_wait();
+    grid_launch_dependents();
+    PagedWalk<kTcItem, kTileKeys, true> walk;
+    const bool any = walk.begin(a, sh.walk, blockIdx.x, gridDim.x);
+
+    if (!any && tid == 0) a.parts[1].open[blockIdx.x].last = -1;
+    // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (any && warp == 8) {
+            load_tiles<D, kStages>(a, walk, sh.ring, ring, &k_map, &v_map, heads_outer, 128);
+        } else if (any && warp == 9) {
+            // -------------------------------------------------- issuer
+            constexpr uint32_t ds = tc_idesc(BF16, kTileKeys, false), dv = tc_idesc(BF16, D, true);
+            uint32_t place0 = 0, stays = 0, turns[2] = {0, 0};
+            while (walk.more()) {
+                PagedItem it;
+                int kt0, kt1, out;
+                walk.take(a, it, kt0, kt1, out);
+                const TileOrder order{it.r1 - it.r0 > 128, kt1 - kt0};
+                tile_wait(sh.ring, &sh.q_full, stays++);
+                auto scores = [&](int t, int j, bool last_use) {  // S_t = Q_t K_j^T
+                    const uint32_t p = place0 + order.key_at(j), s = p % kStages;
+                    tile_wait(sh.ring, &sh.ring.full[s], p / kStages);
+                    tc_fence_after();
+                    if (lane == 0 && !sh.ring.abort) {
+                        const uint32_t q0 = smem_u32(sq) + (order.interleaved ? t * 128 * D * 2 : 0), k0 = smem_u32(ring) + s * kStage;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint32_t at = (k >> 2) * 16384 + (k & 3) * 32;
+                            tc_mma_ss(tmem + t * 128, tc_desc_rows(q0 + at), tc_desc_rows(k0 + at), ds, k > 0);
+                        }
+                        tc_commit(&sh.s_full[t]);
+                        if (last_use) tc_commit(&sh.ring.empty[s]);
+                    }
+                    __syncwarp();
+                };
+                auto values = [&](int t, int j, bool first, bool last, bool first_use, bool last_use) {  // O_t += P_t V_j
+                    const uint32_t p = place0 + order.value_at(j), s = p % kStages;
+                    tile_wait(sh.ring, &sh.ring.full[s], p / kStages);
+                    // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
+                    const int key0 = (kt0 + j) * kTileKeys;
+                    if (first_use && (key0 < it.lo || key0 + kTileKeys > it.hi)) {
+                        for (int i = lane; i < kTileKeys * kBlocks * 8; i += 32) {
+                            const int r = (i >> 3) & (kTileKeys - 1);
+                            if (key0 + r < it.lo || key0 + r >= it.hi)
+                                *reinterpret_cast<uint4 *>(ring + s * kStage + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    tile_wait(sh.ring, &sh.p_full[t], turns[t]++);
+                    tc_fence_after();
+                    if (lane == 0 && !sh.ring.abort) {
+                        const uint32_t v0 = smem_u32(ring) + s * kStage;
+#pragma unroll
+                        for (int k = 0; k < kTileKeys / 16; ++k)
+                            tc_mma_ts(tmem + kO + t * 128, tmem + t * 128 + k * 8, tc_desc_cols(v0 + k * 2048), dv,
+                                      !(first && k == 0));
+                        if (last_use) tc_commit(&sh.ring.empty[s]);
+                        if (last) tc_commit(&sh.o_full[t]);
+                    }
+                    __syncwarp();
+                };
+                const int n = order.n;
+                if (order.interleaved) {
+                    scores(0, 0, false);
+                    scores(1, 0, true);
+                    for (int j = 0; j < n; ++j) {
+                        values(0, j, j == 0, j + 1 == n, true, false);
+                        if (j + 1 < n) scores(0, j + 1, false);
+                        values(1, j, j == 0, j + 1 == n, false, true);
+                        if (j + 1 < n) scores(1, j + 1, true);
+                    }
+                } else {
+                    scores(0, 0, true);
+                    if (n > 1) scores(1, 1, true);
+                    for (int j = 0; j < n; ++j) {
+                        values(j & 1, j, j < 2, j + 2 >= n, true, true);
+                        if (j + 2 < n) scores(j & 1, j + 2, true);
+                    }
+                }
+                place0 += 2 * n;
+            }
+            // every product issued completes before TMEM is freed
+            if (lane == 0) {
+                tc_commit(&sh.drain);
+                mbar_wait_bounded(&sh.drain, 0, kTilePolls);
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // -------------------------------------------------- softmax: a thread to a row
+        const int t = warp >> 2, wrow = (warp & 3) * 32, lrow = wrow + lane;
+        const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16);
+        const uint32_t o_at = s_at - t * 128 + kO + t * 128;
+        const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
+        const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+        uint32_t tiles_seen = 0, ends[2] = {0, 0};
+        while (any && walk.more()) {
+            PagedItem it;
+            int kt0, kt1, out;
+            walk.take(a, it, kt0, kt1, out);
+            const int n = kt1 - kt0, rows = it.r1 - it.r0;
+            if (tid == 0 && !walk.more()) {
+                PagedOpen open{it, -1};
+                if (out >= 0 && (out & 1)) open.last = walk.last_cta(n);
+                a.parts[1].open[blockIdx.x] = open;
+            }
+            const bool both = rows > 128;
+            const int mine = both ? n : (n - t + 1) / 2;  // key tiles of this stream
+            const int row = it.r0 + (both ? t * 128 : 0) + lrow;
+            const bool live = row < it.r1;
+            const bool warp_live = row - lane < it.r1;
+            int lo, hi;
+            paged_row_range(a, it, row, lo, hi);
+            // Q rows into shared memory; with the same rows in both streams each loads half the columns
+            if (!both) asm volatile("bar.sync 1, 256;" ::: "memory");  // both streams have left the last stay
+            {
+                const uint16_t *q = static_cast<const uint16_t *>(a.q) +
+                                    (live ? paged_row_offset(a, it, row, a.q_row, a.q_head) : 0);
+                uint8_t *dst = sq + (both ? t * 128 * D * 2 : 0);
+                const int c0 = both ? 0 : t * (D / 16), c1 = both ? D / 8 : c0 + D / 16;
+#pragma unroll 8
+                for (int i = c0; i < c1; ++i) {
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (live) w = __ldg(reinterpret_cast<const uint4 *>(q + i * 8));
+                    w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
+                    *reinterpret_cast<uint4 *>(dst + (i >> 3) * 16384 + lrow * 128 + (((i & 7) ^ (lrow & 7)) << 4)) = w;
+                }
+            }
+            fence_proxy_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tile_arrive(&sh.q_full);
+
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < mine; ++j) {
+                tile_wait(sh.ring, &sh.s_full[t], tiles_seen++);
+                tc_fence_after();
+                if (warp_live) {
+                    const int key0 = (kt0 + (both ? j : 2 * j + t)) * kTileKeys;
+                    float s[4][32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tc_ld32(s_at + 32 * i, s[i]);
+                    tc_ld_wait();
+                    if (key0 < it.lo_all || key0 + kTileKeys > it.hi_all) {
+                        const int first = lo - key0, last = hi - key0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (32 * i + k < first || 32 * i + k >= last) s[i][k] = -INFINITY;
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        top[i] = s[i][0];
+#pragma unroll
+                        for (int k = 1; k < 32; ++k) top[i] = fmaxf(top[i], s[i][k]);
+                    }
+                    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                    const bool grows = now > m + kTcSlack || m == -INFINITY;
+                    if (__any_sync(0xffffffffu, grows && m != -INFINITY)) {
+                        // S_t of this tile being complete, so is every earlier product of the stream
+                        const float back = grows ? exp2_fast(m - now) : 1.0f;
+                        l *= m == -INFINITY ? 1.0f : back;
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            float o[32];
+                            uint32_t w[32];
+                            tc_ld32(o_at + 32 * i, o);
+                            tc_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(m == -INFINITY ? 0.0f : o[k] * back);
+                            tc_st32(o_at + 32 * i, w);
+                        }
+                    }
+                    if (grows) m = now;
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            float &x = s[2 * i + (k >> 4)][2 * (k & 15)], &y = s[2 * i + (k >> 4)][2 * (k & 15) + 1];
+                            x = exp2_fast(fmaf(x, c, -base));
+                            y = exp2_fast(fmaf(y, c, -base));
+                            sum[k & 3] += x + y;
+                            w[k] = tc_pack<BF16>(x, y);
+                        }
+                        tc_st32(s_at + 32 * i, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tile_arrive(&sh.p_full[t]);
+            }
+            // the end of the stay: this stream's products, and with the same rows the other's too
+            if (both || t == 0 || mine > 0) tile_wait(sh.ring, &sh.o_full[t], ends[t]);
+            if (!both && t == 1) tile_wait(sh.ring, &sh.o_full[0], ends[0]);
+            if (!both && t == 0 && n > 1) tile_wait(sh.ring, &sh.o_full[1], ends[1]);
+            ++ends[0];
+            ends[1] += both || n > 1;
+            tc_fence_after();
+            float4 *swap = reinterpret_cast<float4 *>(sq);  // Q is done with: O of stream 1, [column / 4][row]
+            float mine_w = 1.0f, other_w = 0.0f;
+            if (!both) {
+                if (t == 1 && warp_live) {
+                    sh.ml[lrow] = make_float2(m, l);
+                    if (mine > 0)
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            float o[32];
+                            tc_ld32(o_at + 32 * i, o);
+                            tc_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                swap[(i * 8 + k) * 128 + lrow] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        }
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (t == 0 && warp_live && n > 1) {
+                    const float2 x = sh.ml[lrow];
+                    const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
+                    mine_w = exp2_fast(m - base);
+                    other_w = exp2_fast(x.x - base);
+                    l = l * mine_w + x.y * other_w;
+                    m = top;
+                }
+            }
+            if ((both || t == 0) && warp_live) {
+                const float inv = out >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+                float probe = 0.0f;
+                float *po = a.parts[1].o + (static_cast<int64_t>(max(out, 0)) * kTcItem + row - it.r0) * D;
+                const int64_t at = live ? paged_row_offset(a, it, row, a.out_row, D) : 0;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    float o[32];
+                    tc_ld32(o_at + 32 * i, o);
+                    tc_ld_wait();
+                    if (!both && n > 1) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 x = swap[(i * 8 + k) * 128 + lrow];
+                            o[4 * k] = o[4 * k] * mine_w + x.x * other_w;
+                            o[4 * k + 1] = o[4 * k + 1] * mine_w + x.y * other_w;
+                            o[4 * k + 2] = o[4 * k + 2] * mine_w + x.z * other_w;
+                            o[4 * k + 3] = o[4 * k + 3] * mine_w + x.w * other_w;
+                        }
+                    }
+                    if (out >= 0) {
+                        if (live)
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4)
+                                *reinterpret_cast<float4 *>(po + 32 * i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    } else {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float x = o[2 * k] * inv, y = o[2 * k + 1] * inv;
+                            probe += 0.0f * x + 0.0f * y;
+                            w[k] = tc_pack<BF16>(x, y);
+                        }
+                        if (live)
+#pragma unroll
+                            for (int k = 0; k < 16; k += 4)
+                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at + 32 * i + 2 * k) =
+                                    make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (out >= 0 && live) *reinterpret_cast<float2 *>(a.parts[1].ml + (po - a.parts[1].o) / D * 2) = make_float2(m, l);
+                // rows with a value that is not finite are done again, key by key
+                unsigned odd = __ballot_sync(0xffffffffu, live && out < 0 && !(probe == 0.0f));
+                while (odd) {
+                    const int r = __ffs(odd) - 1;
+                    odd &= odd - 1;
+                    paged_slow_row<D, MODE>(a, it, row - lane + r);
+                }
+            }
+            tc_fence_before();
+            if (!both) asm volatile("bar.sync 1, 256;" ::: "memory");  // the swap area is free
+        }
+    }
+    if (sh.ring.abort && tid == 0) set_flag(a.flags, BD_FLAG_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+    }
+}
+
+template <int D, bool BF16>
+static int launch_tc(const PagedArgs &a, const PagedMaps &maps, int ctas, cudaStream_t stream) {
+    if (cudaFuncSetAttribute(paged_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(tc_smem<D>())) != cudaSuccess)
+        return BD_ERR_LAUNCH;
+    return launch_pdl(paged_tc_kernel<D, BF16>, dim3(ctas), dim3(kTcThreads), tc_smem<D>(), stream, a, maps.k, maps.v,
+                      maps.heads_outer);
+}
+
+int launch_paged_tc(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream) {
+    if (head_dim == 64)
+        return mode == PAGED_BF16 ? launch_tc<64, true>(a, maps, ctas, stream) : launch_tc<64, false>(a, maps, ctas, stream);
+    return mode == PAGED_BF16 ? launch_tc<128, true>(a, maps, ctas, stream) : launch_tc<128, false>(a, maps, ctas, stream);
+}
+
+}  // namespace bd

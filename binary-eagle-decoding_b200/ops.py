@@ -698,6 +698,7 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
 
 
 _PLAN_ROWS = 4096  # rows that the plan's one CTA fills itself
+_SPLIT_ROWS = 64  # rows per kv head from which a request goes to the tcgen05 kernel
 
 
 def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor, flags: Flags | None = None) -> None:
@@ -775,7 +776,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
             window or 0, min(longest or 0, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, _p(out),
             int(fresh), _p(ws), nbytes, flags.ptr,
         )
-        _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device))
+        both = q.dtype != torch.float32 and min(longest or rows, rows) * (heads // kv_heads) > _SPLIT_ROWS
+        _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device), kernels=2 + both)
         if own:
             flags.check()
     return out
