@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import re
+import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -88,6 +89,11 @@ class PagedAttentionArgs(ctypes.Structure):
         ("head_dim", c_int), ("causal", c_int), ("window", c_int64), ("longest", c_int), ("scale", ctypes.c_float),
         ("out", P), ("zero_fill", c_int), ("workspace", P), ("workspace_bytes", c_size_t), ("flags", P),
     ]
+
+
+# the same, packed at once (native alignment)
+PAGED_ATTENTION_ARGS = struct.Struct("@PqqiPP3q3qiiqPqiPPiqiiiiqifPiPNP")
+assert PAGED_ATTENTION_ARGS.size == ctypes.sizeof(PagedAttentionArgs)
 
 
 SIGNATURES = {

@@ -8,7 +8,6 @@ caller, for deferred checks) reads them.
 
 from __future__ import annotations
 
-import contextlib
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -594,6 +593,7 @@ def argmax_rows(logits: Tensor, flags: Flags | None = None) -> Tensor:
 # --------------------------------------------------------------------------- paged cache
 
 _ROW_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_CACHE_TYPE = {torch.float16: 0, torch.bfloat16: 1}
 _ATTENDS = {(torch.float32, torch.float16), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)}
 PAGE_SIZES = (8, 16, 32, 64, 128, 256)
 
@@ -607,48 +607,37 @@ class PagePlan(NamedTuple):
     slots: Tensor
 
 
-def _same_device(*tensors: Tensor) -> torch.device:
-    device = tensors[0].device
-    if device.type != "cuda":
-        raise ValueError("bitdraft kernels take CUDA tensors")
-    for t in tensors:
-        if t.device != device:
-            raise ValueError("all tensors must be on one device")
-    return device
-
-
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch (its streams and kernels belong to it)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def _int32(name: str, t: Tensor, *shape: int) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+def _int32(name: str, t: Tensor, shape: tuple[int, ...]) -> None:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}")
 
 
-def _check_table(table: Tensor, requests: int) -> None:
-    if table.dtype != torch.int32 or table.ndim != 2 or table.shape[0] != requests or table.shape[1] < 1 \
-            or (table.shape[1] > 1 and table.stride(1) != 1) or (requests > 1 and table.stride(0) < table.shape[1]):
-        raise ValueError("table must be int32 [requests, pages of a request] with unit column stride")
+def _table_ld(table: Tensor, requests: int) -> int:
+    """The row stride of a table of pages."""
+    shape = table.shape
+    if table.dtype is torch.int32 and len(shape) == 2 and shape[0] == requests and shape[1] > 0:
+        row, column = table.stride()
+        if (column == 1 or shape[1] == 1) and (row >= shape[1] or requests < 2):
+            return max(row, shape[1])
+    raise ValueError("table must be int32 [requests, pages of a request] with unit column stride")
 
 
-def _table_ld(table: Tensor) -> int:
-    return max(table.stride(0), table.shape[1])
-
-
-def _check_caches(k_cache: Tensor, v_cache: Tensor) -> None:
-    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype \
-            or k_cache.dtype not in (torch.float16, torch.bfloat16):
+def _cache_shape(k_cache: Tensor, v_cache: Tensor) -> torch.Size:
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype is not v_cache.dtype or k_cache.dtype not in _CACHE_TYPE:
         raise ValueError("caches must be fp16 or bf16 [pages, page_size, kv_heads, head_dim], both alike")
-    if k_cache.shape[0] < 1 or k_cache.shape[1] not in PAGE_SIZES:
+    if shape[0] < 1 or shape[1] not in PAGE_SIZES:
         raise ValueError("page_size must be a power of two from 8 to 256, in at least one page")
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
-        raise ValueError("caches need unit stride within a head")
+    return shape
 
 
-def _strides(cache: Tensor):
-    return (_lib.c_int64 * 3)(*cache.stride()[:3])
+def _one_device(device: torch.device, *others: Tensor) -> None:
+    if device.type != "cuda":
+        raise ValueError("bitdraft kernels take CUDA tensors")
+    index = device.index
+    for t in others:
+        if t.get_device() != index:
+            raise ValueError("all tensors must be on one device")
 
 
 def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free: Tensor, top: Tensor, page_size: int,
@@ -666,34 +655,43 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
     ``top_out`` are given.  Returns ``starts [B + 1]`` and, for ``rows`` rows,
     ``positions`` and ``slots`` (-1 behind the last request).  Without ``flags`` the
     call waits and raises ``ValueError`` for lengths that do not fit or a lack of pages."""
-    requests = context.shape[0] if context.ndim == 1 else 0
+    requests = context.shape[0] if context.dim() == 1 else 0
     if requests < 1:
         raise ValueError("a plan needs int32 lengths of at least one request")
-    _int32("context", context, requests)
-    _int32("count", count, requests)
-    _int32("owned", owned, requests)
-    _int32("top", top, 1)
-    _int32("free", free, free.numel())
-    owned_out = owned if owned_out is None else owned_out
-    top_out = top if top_out is None else top_out
-    _int32("owned_out", owned_out, requests)
-    _int32("top_out", top_out, 1)
-    _check_table(table, requests)
+    shape = (requests,)
+    _int32("context", context, shape)
+    _int32("count", count, shape)
+    _int32("owned", owned, shape)
+    _int32("top", top, (1,))
+    capacity = free.numel()
+    _int32("free", free, (capacity,))
+    if owned_out is None:
+        owned_out = owned
+    else:
+        _int32("owned_out", owned_out, shape)
+    if top_out is None:
+        top_out = top
+    else:
+        _int32("top_out", top_out, (1,))
+    ld = _table_ld(table, requests)
     if page_size not in PAGE_SIZES:
         raise ValueError("page_size must be a power of two from 8 to 256")
     if rows < 0:
         raise ValueError("rows must not be negative")
-    device = _same_device(context, count, table, owned, free, top, owned_out, top_out)
-    with _on(device):
-        out = torch.empty(requests + 1 + 2 * rows, dtype=torch.int32, device=device)
-        starts, positions, slots = out[:requests + 1], out[requests + 1:requests + 1 + rows], out[requests + 1 + rows:]
-        own = flags is None
-        flags = flags or Flags(device)
-        _lib.call("bd_page_plan", _p(context), _p(count), requests, page_size, pool_pages, _p(table), _table_ld(table),
-                  table.shape[1], _p(owned), _p(owned_out), _p(free), free.numel(), _p(top), _p(top_out), _p(starts),
-                  _p(positions), _p(slots), rows, flags.ptr, _stream(device), kernels=1 + (rows > _PLAN_ROWS))
-        if own:
-            flags.check()
+    device = context.device
+    _one_device(device, count, table, owned, free, top, owned_out, top_out)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return page_plan(context, count, table, owned, free, top, page_size, rows, pool_pages, owned_out, top_out, flags)
+    starts, positions, slots = context.new_empty(requests + 1), context.new_empty(rows), context.new_empty(rows)
+    own = flags is None
+    flags = flags or Flags(device)
+    _lib.call("bd_page_plan", context.data_ptr(), count.data_ptr(), requests, page_size, pool_pages, table.data_ptr(), ld,
+              table.shape[1], owned.data_ptr(), owned_out.data_ptr(), free.data_ptr(), capacity, top.data_ptr(),
+              top_out.data_ptr(), starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), rows, flags.ptr,
+              _stream(device), kernels=1 if rows <= _PLAN_ROWS else 2)
+    if own:
+        flags.check()
     return PagePlan(starts, positions, slots)
 
 
@@ -707,23 +705,34 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
     ``[pages, page_size, kv_heads, head_dim]``, rounded to their type.  Rows with slot -1 are
     skipped; a slot may appear once.  Raises (or flags) "F16 cache storage overflow"
     when a stored value is not finite."""
-    _check_caches(k_cache, v_cache)
-    rows = k.shape[0] if k.ndim == 3 else -1
-    if rows < 0 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ROW_TYPE or k.shape[1:] != k_cache.shape[2:]:
+    pages, page_size, kv_heads, head_dim = _cache_shape(k_cache, v_cache)
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or shape != v.shape or dtype is not v.dtype or dtype not in _ROW_TYPE or shape[1] != kv_heads \
+            or shape[2] != head_dim:
         raise ValueError("k and v must be fp32, fp16 or bf16 [rows, kv_heads, head_dim] of the caches' heads")
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    (k_row, k_head, k_one), (v_row, v_head, v_one) = k.stride(), v.stride()
+    (*k_strides, kc_one), (*v_strides, vc_one) = k_cache.stride(), v_cache.stride()
+    if kc_one != 1 or vc_one != 1:
+        raise ValueError("caches need unit stride within a head")
+    if k_one != 1 or v_one != 1:
         raise ValueError("k and v need unit stride within a head")
-    _int32("slots", slots, rows)
-    device = _same_device(k, v, slots, k_cache, v_cache)
-    with _on(device):
-        own = flags is None
-        flags = flags or Flags(device)
-        pages, page_size, kv_heads, head_dim = k_cache.shape
-        _lib.call("bd_paged_store", _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _ROW_TYPE[k.dtype],
-                  _p(slots), rows, kv_heads, head_dim, page_size, pages, _p(k_cache), _strides(k_cache), _p(v_cache),
-                  _strides(v_cache), _ROW_TYPE[k_cache.dtype], flags.ptr, _stream(device))
-        if own:
-            flags.check()
+    rows = shape[0]
+    _int32("slots", slots, (rows,))
+    device = k.device
+    _one_device(device, v, slots, k_cache, v_cache)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return paged_store(k, v, slots, k_cache, v_cache, flags)
+    own = flags is None
+    flags = flags or Flags(device)
+    _lib.call("bd_paged_store", k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, _ROW_TYPE[dtype],
+              slots.data_ptr(), rows, kv_heads, head_dim, page_size, pages, k_cache.data_ptr(), _Strides(*k_strides),
+              v_cache.data_ptr(), _Strides(*v_strides), _CACHE_TYPE[k_cache.dtype], flags.ptr, _stream(device))
+    if own:
+        flags.check()
+
+
+_Strides = _lib.c_int64 * 3
 
 
 def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, context: Tensor, starts: Tensor,
@@ -740,44 +749,54 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
     ``longest``: an upper bound of the requests' new tokens, when the caller knows
     one.  Returns ``out``, whose rows of no request stay as they were; without ``out``
     a new tensor in which they are zero."""
-    _check_caches(k_cache, v_cache)
-    if q.ndim != 3 or (q.dtype, k_cache.dtype) not in _ATTENDS:
+    pages, page_size, kv_heads, cache_dim = _cache_shape(k_cache, v_cache)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or (dtype, k_cache.dtype) not in _ATTENDS:
         raise ValueError("q must be [rows, heads, head_dim]: fp32 or fp16 over fp16 caches, bf16 over bf16")
-    rows, heads, head_dim = q.shape
-    pages, page_size, kv_heads, cache_dim = k_cache.shape
+    rows, heads, head_dim = shape
     if head_dim != cache_dim or head_dim not in (64, 128) or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("head_dim must be 64 or 128, the caches' own, and heads a multiple of kv_heads")
-    if q.stride(2) != 1:
+    (q_row, q_head, q_one), k_strides, v_strides = q.stride(), k_cache.stride(), v_cache.stride()
+    if k_strides[3] != 1 or v_strides[3] != 1:
+        raise ValueError("caches need unit stride within a head")
+    if q_one != 1:
         raise ValueError("q needs unit stride within a head")
-    requests = context.shape[0] if context.ndim == 1 else 0
-    _int32("context", context, requests)
-    _int32("starts", starts, requests + 1)
-    _check_table(table, requests)
-    if window is not None and window < 1:
+    requests = context.numel()
+    _int32("context", context, (requests,))
+    _int32("starts", starts, (requests + 1,))
+    ld = _table_ld(table, requests)
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError("window must be at least 1")
-    if longest is not None and longest < 1:
+    if longest is None:
+        longest = rows
+    elif longest < 1:
         raise ValueError("longest must be at least 1")
-    device = _same_device(q, k_cache, v_cache, table, context, starts)
+    device = q.device
+    _one_device(device, k_cache, v_cache, table, context, starts)
     fresh = out is None
-    if not fresh and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
+    if not fresh and (out.shape != shape or out.dtype is not dtype or out.device != device or not out.is_contiguous()):
         raise ValueError("out must be contiguous and like q")
-    with _on(device):
-        if fresh:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        nbytes = _lib.size("bd_paged_attention_workspace_bytes", head_dim)
-        # a buffer of this call: concurrent streams and captured graphs share none
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        own = flags is None
-        flags = flags or Flags(device)
-        args = _lib.PagedAttentionArgs(
-            _p(q), q.stride(0), q.stride(1), _ROW_TYPE[q.dtype], _p(k_cache), _p(v_cache), k_cache.stride()[:3],
-            v_cache.stride()[:3], _ROW_TYPE[k_cache.dtype], page_size, pages, _p(table), _table_ld(table),
-            table.shape[1], _p(context), _p(starts), requests, rows, heads, kv_heads, head_dim, int(causal),
-            window or 0, min(longest or 0, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, _p(out),
-            int(fresh), _p(ws), nbytes, flags.ptr,
-        )
-        both = q.dtype != torch.float32 and min(longest or rows, rows) * (heads // kv_heads) > _SPLIT_ROWS
-        _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device), kernels=2 + both)
-        if own:
-            flags.check()
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return paged_attention(q, k_cache, v_cache, table, context, starts, causal, window or None, scale, longest or 1,
+                                   out, flags)
+    if fresh:
+        out = q.new_empty(shape)
+    nbytes = _lib.size("bd_paged_attention_workspace_bytes", head_dim)
+    # a buffer of this call: concurrent streams and captured graphs share none
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    own = flags is None
+    flags = flags or Flags(device)
+    args = _lib.PagedAttentionArgs.from_buffer_copy(_lib.PAGED_ATTENTION_ARGS.pack(
+        q.data_ptr(), q_row, q_head, _ROW_TYPE[dtype], k_cache.data_ptr(), v_cache.data_ptr(), *k_strides[:3],
+        *v_strides[:3], _CACHE_TYPE[k_cache.dtype], page_size, pages, table.data_ptr(), ld, table.shape[1],
+        context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
+        min(longest, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
+        flags.ptr))
+    both = dtype is not torch.float32 and min(longest, rows) * (heads // kv_heads) > _SPLIT_ROWS
+    _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device), kernels=2 + both)
+    if own:
+        flags.check()
     return out
