@@ -242,7 +242,7 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     a.requests = p->requests;
     a.rows = p->rows;
     a.kv_heads = p->kv_heads;
-    a.groups = p->heads / p->kv_heads;
+    paged_set_groups(a, p->heads / p->kv_heads);
     a.page_shift = log2_of(p->page_size);
     a.causal = p->causal != 0;
     a.window = p->window > INT32_MAX ? 0 : static_cast<int>(p->window);

@@ -28,6 +28,7 @@ struct PagedArgs {
     int requests;
     int64_t rows;  // rows of q and out
     int kv_heads, groups, page_shift;
+    uint32_t group_mul, group_shift;  // row / groups, see paged_token()
     int causal, window, longest;  // window 0: none
     float scale_log2;             // scale x log2 e
     void *out;
@@ -46,6 +47,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// row / groups for 0 <= row < 2^31: with 2^(s-1) < groups <= 2^s and the multiplier
+// m = ceil(2^(31+s) / groups) < 2^32, row m 2^-(31+s) exceeds row / groups by less than
+// row 2^-(31+s) < 1 / groups, so the floors agree.
+__device__ __forceinline__ int paged_token(const PagedArgs &a, int row) {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(row)) * a.group_mul) >> a.group_shift);
+}
+inline void paged_set_groups(PagedArgs &a, int groups) {
+    int s = 0;
+    while ((1 << s) < groups) ++s;
+    a.groups = groups;
+    a.group_shift = 31 + s;
+    a.group_mul = static_cast<uint32_t>(((uint64_t{1} << (31 + s)) + groups - 1) / groups);
 }
 
 // A request's lengths; one whose lengths do not fit has no tokens.
@@ -92,13 +107,13 @@ __device__ __forceinline__ void paged_item(const PagedArgs &a, const PagedReques
     it.context = r.context;
     it.r0 = i * M;
     it.r1 = min(it.r0 + M, r.count * a.groups);
-    paged_token_range(a, r.context, r.count, it.r0 / a.groups, it.lo, it.hi_all);
-    paged_token_range(a, r.context, r.count, (it.r1 - 1) / a.groups, it.lo_all, it.hi);
+    paged_token_range(a, r.context, r.count, paged_token(a, it.r0), it.lo, it.hi_all);
+    paged_token_range(a, r.context, r.count, paged_token(a, it.r1 - 1), it.lo_all, it.hi);
 }
 
 __device__ __forceinline__ void paged_row_range(const PagedArgs &a, const PagedItem &it, int row, int &lo, int &hi) {
     if (row < it.r1) {
-        paged_token_range(a, it.context, it.count, row / a.groups, lo, hi);
+        paged_token_range(a, it.context, it.count, paged_token(a, row), lo, hi);
     } else {
         lo = hi = 0;
     }
@@ -107,7 +122,7 @@ __device__ __forceinline__ void paged_row_range(const PagedArgs &a, const PagedI
 // Element offset of a row in a tensor of the given token and head strides.
 __device__ __forceinline__ int64_t paged_row_offset(const PagedArgs &a, const PagedItem &it, int row, int64_t token_stride,
                                                     int64_t head_stride) {
-    const int t = row / a.groups;
+    const int t = paged_token(a, row);
     return (static_cast<int64_t>(it.row0) + t) * token_stride +
            (static_cast<int64_t>(it.h) * a.groups + (row - t * a.groups)) * head_stride;
 }
@@ -121,17 +136,19 @@ struct PagedOpen {
 
 struct PagedShared {
     int64_t warp_sums[32];
-    int64_t before;
+    int64_t before, each;
     int b;
 };
 
-// The walk over the units of this CTA's range, see the head of paged_attention.cu: the
+// The walk over this CTA's range of the batch, see the head of paged_attention.cu: the
 // items of M rows and units of KT keys of the requests of one kernel (TC: those of
-// more than a.split_rows rows per kv head, else the others).
-template <int M, int KT, bool TC>
+// more than a.split_rows rows per kv head, else the others).  An item counts as its
+// units and EXTRA more, which is what a stay costs beside its tiles; a range that
+// ends within these leaves the item to the next CTA.
+template <int M, int KT, int EXTRA, bool TC>
 struct PagedWalk {
-    int cta, at, len, per;      // this CTA's range: units done, in all, and of every CTA's range but the last
-    int off;                    // units of the current item before the range
+    int cta, len, per;          // this CTA's range, and that of every CTA but the last
+    int at;                     // where the current item begins, counted from the range's begin (first: <= 0)
     int b, h, i, tiles, units;  // units: of the item
     PagedRequest r;
 
@@ -140,17 +157,35 @@ struct PagedWalk {
         const int rows = r.count * a.groups;
         return (rows > a.split_rows) == TC ? (rows + M - 1) / M : 0;
     }
+    static __device__ __forceinline__ int cost(const PagedArgs &a, const PagedRequest &r, int i) {
+        PagedItem x;
+        paged_item<M>(a, r, i, x);
+        return item_units(x) + EXTRA;
+    }
 
-    // Units of one kv head of request b.
-    static __device__ __forceinline__ int64_t request_units(const PagedArgs &a, int b) {
-        const PagedRequest r = paged_request(a, b);
-        if (r.bad) set_flag(a.flags, BD_FLAG_BAD_LENGTH);
-        const int tiles = request_tiles(a, r);
+    // Cost of one kv head of request b, a request to a lane; those of many items by the whole warp.
+    static __device__ __forceinline__ int64_t request_cost(const PagedArgs &a, int b) {
+        PagedRequest r{};
+        if (b < a.requests) {
+            r = paged_request(a, b);
+            if (r.bad) set_flag(a.flags, BD_FLAG_BAD_LENGTH);
+        }
+        const int tiles = b < a.requests ? request_tiles(a, r) : 0;
         int64_t sum = 0;
-        for (int i = 0; i < tiles; ++i) {
-            PagedItem x;
-            paged_item<M>(a, r, i, x);
-            sum += item_units(x);
+        if (tiles <= 4)
+            for (int i = 0; i < tiles; ++i) sum += cost(a, r, i);
+        const int lane = threadIdx.x & 31;
+        for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
+            const int src = __ffs(many) - 1;
+            PagedRequest q{};
+            q.count = __shfl_sync(0xffffffffu, r.count, src);
+            q.context = __shfl_sync(0xffffffffu, r.context, src);
+            const int n = __shfl_sync(0xffffffffu, tiles, src);
+            int64_t part = 0;
+            for (int i = lane; i < n; i += 32) part += cost(a, q, i);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+            if (lane == src) sum = part;
         }
         return sum;
     }
@@ -179,39 +214,33 @@ struct PagedWalk {
         r = paged_request(a, b);
         tiles = request_tiles(a, r);
     }
-    __device__ __forceinline__ void set_item(const PagedArgs &a, PagedItem &it) {
-        paged_item<M>(a, r, i, it);
-        it.b = b;
-        it.h = h;
-        units = item_units(it);
-    }
 
-    // Places the walk at unit `cta x per` of `ctas` equal ranges; false when the range is empty.
+    // Places the walk at the begin of this CTA's range of `ctas` equal ones; false when it is empty.
     __device__ __forceinline__ bool begin(const PagedArgs &a, PagedShared &sh, int cta_, int ctas) {
         cta = cta_;
-        const int n = blockDim.x, tid = threadIdx.x;
-        int64_t w = tid < a.requests ? request_units(a, tid) * a.kv_heads : 0, total, sum;
-        int64_t incl = scan(w, sh, total);
+        const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31;
+        int64_t each = request_cost(a, tid), total, sum;
+        int64_t incl = scan(each * a.kv_heads, sh, total);
         for (int b0 = n; b0 < a.requests; b0 += n) {
-            scan(b0 + tid < a.requests ? request_units(a, b0 + tid) * a.kv_heads : 0, sh, sum);
+            scan(request_cost(a, b0 + tid) * a.kv_heads, sh, sum);
             total += sum;
         }
         per = static_cast<int>((total + ctas - 1) / ctas);
         const int64_t u = static_cast<int64_t>(cta) * per;
         if (u >= total) return false;
-        at = 0;
         len = static_cast<int>(min(static_cast<int64_t>(per), total - u));
-        // the request that holds unit u
+        // the request around u
         int64_t before = 0;
         sum = total;
         for (int b0 = 0; b0 < a.requests; b0 += n) {
             if (a.requests > n) {
-                w = b0 + tid < a.requests ? request_units(a, b0 + tid) * a.kv_heads : 0;
-                incl = scan(w, sh, sum);
+                each = request_cost(a, b0 + tid);
+                incl = scan(each * a.kv_heads, sh, sum);
             }
-            if (before + incl - w <= u && u < before + incl) {
+            if (before + incl - each * a.kv_heads <= u && u < before + incl) {
                 sh.b = b0 + tid;
-                sh.before = before + incl - w;
+                sh.before = before + incl - each * a.kv_heads;
+                sh.each = each;
             }
             before += sum;
             if (u < before) break;
@@ -220,51 +249,64 @@ struct PagedWalk {
         b = sh.b;
         int64_t rest = u - sh.before;
         set_request(a);
-        // its kv head and rows
-        int64_t each = 0;
-        PagedItem it;
-        for (int j = 0; j < tiles; ++j) {
-            paged_item<M>(a, r, j, it);
-            each += item_units(it);
+        // its kv head, and the item: 32 at a time, every warp for itself
+        h = static_cast<int>(rest / sh.each);
+        rest -= h * sh.each;
+        for (int i0 = 0;; i0 += 32) {
+            const int mine = i0 + lane < tiles ? cost(a, r, i0 + lane) : 0;
+            int end = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, end, d);
+                if (lane >= d) end += o;
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, rest < end);
+            if (found) {
+                const int src = __ffs(found) - 1;
+                i = i0 + src;
+                at = -static_cast<int>(rest - __shfl_sync(0xffffffffu, end - mine, src));
+                break;
+            }
+            rest -= __shfl_sync(0xffffffffu, end, 31);
+            if (i0 + 32 >= tiles) return false;  // not reached: the request holds u
         }
-        h = static_cast<int>(rest / each);
-        rest -= h * each;
-        for (i = 0;; ++i) {
-            set_item(a, it);
-            if (rest < units) break;
-            rest -= units;
-        }
-        off = static_cast<int>(rest);
         return true;
     }
 
-    __device__ __forceinline__ bool more() const { return at < len; }
-
     // The next stay: an item, its key tiles [kt0, kt1), and the place of the partial it
     // leaves (-1: it is done whole).  An odd place is an item that later CTAs end.
-    __device__ __forceinline__ void take(const PagedArgs &a, PagedItem &it, int &kt0, int &kt1, int &part) {
-        set_item(a, it);
-        const int n = min(units - off, len - at);
-        kt0 = it.lo / KT + off;
-        kt1 = kt0 + n;
-        part = off == 0 && n == units ? -1 : 2 * cta + (off == 0);
-        at += n;
-        if (at >= len) return;
-        off = 0;
-        if (++i == tiles) {
-            i = 0;
-            if (++h == a.kv_heads) {
-                h = 0;
-                do {
-                    ++b;
-                    set_request(a);
-                } while (tiles == 0);
+    // False at the end of the range.
+    __device__ __forceinline__ bool next(const PagedArgs &a, PagedItem &it, int &kt0, int &kt1, int &part) {
+        while (at < len) {
+            if (i == tiles) {
+                i = 0;
+                if (++h == a.kv_heads) {
+                    h = 0;
+                    do {
+                        ++b;
+                        set_request(a);
+                    } while (tiles == 0);
+                }
+            }
+            paged_item<M>(a, r, i, it);
+            it.b = b;
+            it.h = h;
+            units = item_units(it);
+            const int first = max(0, -at - EXTRA), last = min(units, len - at - EXTRA);
+            at += units + EXTRA;
+            ++i;
+            if (first < last) {
+                kt0 = it.lo / KT + first;
+                kt1 = it.lo / KT + last;
+                part = first == 0 && last == units ? -1 : 2 * cta + (first == 0);
+                return true;
             }
         }
+        return false;
     }
 
-    // The CTA that ends the item of the last stay, which began at its first unit with n units here.
-    __device__ __forceinline__ int last_cta(int n) const { return cta + (at - n + units - 1) / per; }
+    // The CTA that ends the item of the last stay.
+    __device__ __forceinline__ int last_cta() const { return cta + (at - 1) / per; }
 };
 
 // One row by one warp, key by key: for rows whose tile products met values that are
@@ -401,10 +443,9 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
     const int pieces = kTileKeys / piece;
     const int block = lane / pieces, part = lane - block * pieces;
     uint32_t place = 0;
-    while (walk.more()) {
-        PagedItem it;
-        int kt0, kt1, out;
-        walk.take(a, it, kt0, kt1, out);
+    PagedItem it;
+    int kt0, kt1, out;
+    while (walk.next(a, it, kt0, kt1, out)) {
         const TileOrder order{it.r1 - it.r0 > alternating_rows, kt1 - kt0};
         const int32_t *table = a.table + it.b * a.table_ld;
         int next_key = 0, next_value = 0;

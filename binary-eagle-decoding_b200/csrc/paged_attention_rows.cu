@@ -15,6 +15,7 @@
 namespace bd {
 
 constexpr int kRowsWarps = 8;
+constexpr int kRowsExtra = 1;  // a stay's Q, joining and output, in units
 constexpr int kRowsThreads = 384;  // the last three warps only lend their registers
 
 template <int D>
@@ -391,11 +392,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     __syncthreads();
     grid_wait();
     grid_launch_dependents();
-    PagedWalk<kRowsItem, kTileKeys, false> walk;
-    if (!walk.begin(a, sh.walk, blockIdx.x, gridDim.x)) {
-        if (tid == 0) a.parts[0].open[blockIdx.x].last = -1;
-        return;
-    }
+    PagedWalk<kRowsItem, kTileKeys, kRowsExtra, false> walk;
+    if (tid == 0) a.parts[0].open[blockIdx.x].last = -1;
+    if (!walk.begin(a, sh.walk, blockIdx.x, gridDim.x)) return;
     // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
     if (warp >= kRowsWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -403,16 +402,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         uint32_t place = 0;
-        while (walk.more()) {
-            PagedItem it;
-            int kt0, kt1, part;
-            walk.take(a, it, kt0, kt1, part);
+        PagedItem it;
+        int kt0, kt1, part;
+        while (walk.next(a, it, kt0, kt1, part)) {
             const int rows = it.r1 - it.r0;
-            if (tid == 0 && !walk.more()) {
-                PagedOpen open{it, -1};
-                if (part >= 0 && (part & 1)) open.last = walk.last_cta(kt1 - kt0);
-                a.parts[0].open[blockIdx.x] = open;
-            }
+            if (tid == 0 && part >= 0 && (part & 1)) a.parts[0].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
             if (rows <= 16)
                 rows_stay<D, MODE, 1>(a, it, kt0, kt1, part, sh, stages, area, place);
             else if (rows <= 32)

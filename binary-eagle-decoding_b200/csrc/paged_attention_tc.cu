@@ -25,6 +25,7 @@
 namespace bd {
 
 constexpr int kTcThreads = 384;  // warps 10 and 11 only lend their registers
+constexpr int kTcExtra = 3;       // a stay's Q, first and last products and output, in units
 constexpr float kTcSlack = 8.0f;  // growth of a maximum (log2) that leaves O as it is
 
 template <int D>
@@ -110,6 +111,12 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         : "memory");
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
     if (BF16) {
@@ -157,10 +164,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = sh.tmem;
     grid_wait();
     grid_launch_dependents();
-    PagedWalk<kTcItem, kTileKeys, true> walk;
+    PagedWalk<kTcItem, kTileKeys, kTcExtra, true> walk;
+    if (tid == 0) a.parts[1].open[blockIdx.x].last = -1;
     const bool any = walk.begin(a, sh.walk, blockIdx.x, gridDim.x);
-
-    if (!any && tid == 0) a.parts[1].open[blockIdx.x].last = -1;
     // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -170,10 +176,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // -------------------------------------------------- issuer
             constexpr uint32_t ds = tc_idesc(BF16, kTileKeys, false), dv = tc_idesc(BF16, D, true);
             uint32_t place0 = 0, stays = 0, turns[2] = {0, 0};
-            while (walk.more()) {
-                PagedItem it;
-                int kt0, kt1, out;
-                walk.take(a, it, kt0, kt1, out);
+            PagedItem it;
+            int kt0, kt1, out;
+            while (walk.next(a, it, kt0, kt1, out)) {
                 const TileOrder order{it.r1 - it.r0 > 128, kt1 - kt0};
                 tile_wait(sh.ring, &sh.q_full, stays++);
                 auto scores = [&](int t, int j, bool last_use) {  // S_t = Q_t K_j^T
@@ -255,16 +260,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
         uint32_t tiles_seen = 0, ends[2] = {0, 0};
-        while (any && walk.more()) {
-            PagedItem it;
-            int kt0, kt1, out;
-            walk.take(a, it, kt0, kt1, out);
+        PagedItem it;
+        int kt0, kt1, out;
+        while (any && walk.next(a, it, kt0, kt1, out)) {
             const int n = kt1 - kt0, rows = it.r1 - it.r0;
-            if (tid == 0 && !walk.more()) {
-                PagedOpen open{it, -1};
-                if (out >= 0 && (out & 1)) open.last = walk.last_cta(n);
-                a.parts[1].open[blockIdx.x] = open;
-            }
+            if (tid == 0 && out >= 0 && (out & 1)) a.parts[1].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
             const bool both = rows > 128;
             const int mine = both ? n : (n - t + 1) / 2;  // key tiles of this stream
             const int row = it.r0 + (both ? t * 128 : 0) + lrow;
@@ -278,13 +278,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint16_t *q = static_cast<const uint16_t *>(a.q) +
                                     (live ? paged_row_offset(a, it, row, a.q_row, a.q_head) : 0);
                 uint8_t *dst = sq + (both ? t * 128 * D * 2 : 0);
-                const int c0 = both ? 0 : t * (D / 16), c1 = both ? D / 8 : c0 + D / 16;
-#pragma unroll 8
-                for (int i = c0; i < c1; ++i) {
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (live) w = __ldg(reinterpret_cast<const uint4 *>(q + i * 8));
-                    w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
-                    *reinterpret_cast<uint4 *>(dst + (i >> 3) * 16384 + lrow * 128 + (((i & 7) ^ (lrow & 7)) << 4)) = w;
+                const int c0 = both ? 0 : t * (D / 16);
+                uint4 w[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    w[i] = live && (both || i < D / 16) ? __ldg(reinterpret_cast<const uint4 *>(q + (c0 + i) * 8))
+                                                        : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const int c = c0 + i;
+                    if (both || i < D / 16)
+                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + lrow * 128 + (((c & 7) ^ (lrow & 7)) << 4)) =
+                            make_uint4(w[i].x ^ flip, w[i].y ^ flip, w[i].z ^ flip, w[i].w ^ flip);
                 }
             }
             fence_proxy_async_smem();
@@ -313,9 +318,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     float top[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        top[i] = s[i][0];
+                        top[i] = fmaxf(s[i][0], s[i][1]);
 #pragma unroll
-                        for (int k = 1; k < 32; ++k) top[i] = fmaxf(top[i], s[i][k]);
+                        for (int k = 2; k < 32; k += 2) top[i] = max3(top[i], s[i][k], s[i][k + 1]);
                     }
                     const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
                     const bool grows = now > m + kTcSlack || m == -INFINITY;
@@ -336,21 +341,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     if (grows) m = now;
                     const float base = m == -INFINITY ? 0.0f : m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
+                    float2 sum[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint32_t w[32];
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
-                            float &x = s[2 * i + (k >> 4)][2 * (k & 15)], &y = s[2 * i + (k >> 4)][2 * (k & 15) + 1];
-                            x = exp2_fast(fmaf(x, c, -base));
-                            y = exp2_fast(fmaf(y, c, -base));
-                            sum[k & 3] += x + y;
-                            w[k] = tc_pack<BF16>(x, y);
+                            const float *x = &s[2 * i + (k >> 4)][2 * (k & 15)];
+                            float2 p = __ffma2_rn(make_float2(x[0], x[1]), c2, base2);
+                            p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
+                            sum[k & 3] = __fadd2_rn(sum[k & 3], p);
+                            w[k] = tc_pack<BF16>(p.x, p.y);
                         }
                         tc_st32(s_at + 32 * i, w);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+                    l += all.x + all.y;
                     tc_st_wait();
                 }
                 tc_fence_before();
