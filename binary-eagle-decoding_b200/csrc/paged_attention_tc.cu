@@ -45,8 +45,12 @@ struct TcShared {
     PagedShared walk;
 };
 
-__device__ __forceinline__ void tc_commit(uint64_t *b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+__device__ __forceinline__ void tc_commit(uint64_t *b, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(b)),
+        "r"(leader)
+        : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -81,35 +85,46 @@ __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory operands are 128-byte-swizzled rows of 64 values; a tile of D
-// columns is D / 64 such blocks of 128 rows (16 KB) one behind the other.
-// K-major (Q, K): 8-row groups 1024 B apart, a step of 16 columns is 32 B.
-__device__ __forceinline__ uint64_t tc_desc_rows(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
-}
-// MN-major (V, whose rows are the reduction): 64-column blocks 16 KB apart, 8-row
-// groups 1024 B apart, a step of 16 rows is 2 KB.
-__device__ __forceinline__ uint64_t tc_desc_cols(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(16384 >> 4) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// columns is D / 64 such blocks of 128 rows (16 KB) one behind the other.  The lower
+// word of a matrix descriptor is the address and the leading offset, the upper one is
+// the same for all: 8-row groups 1024 B apart, 128-byte swizzle.
+// K-major (Q, K): a step of 16 columns is 32 B; the leading offset is not used.
+// MN-major (V, whose rows are the reduction): 64-column blocks 16 KB apart, a step of
+// 16 rows is 2 KB.
+constexpr uint32_t kTcDescUpper = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t tc_desc_rows(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t tc_desc_cols(uint32_t addr) { return (addr >> 4) | ((16384u >> 4) << 16); }
 // kind::f16 instruction descriptor: fp32 accumulators, M = 128, A and B fp16 or bf16.
 __host__ __device__ constexpr uint32_t tc_idesc(bool bf16, int n, bool b_cols) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_cols ? 1u : 0u) << 16) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One MMA, issued by the lane whose `leader` is set.  The whole warp runs the code
+// around it, so that its operands can be warp-uniform registers.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.u32 p, %5, 0;\n setp.ne.u32 q, %6, 0;\n"
+        " mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(kTcDescUpper), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.u32 p, %5, 0;\n setp.ne.u32 q, %6, 0;\n"
+        " mov.b64 b, {%2, %3};\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(kTcDescUpper), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
+__device__ __forceinline__ uint32_t tc_elect() {
+    uint32_t leader;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
+    return leader;
+}
+// A value that is the same in all lanes, as one the compiler knows to be.
+__device__ __forceinline__ uint32_t tc_uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float m;
@@ -138,7 +153,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = sq + 2 * 128 * D * 2;
     __shared__ TcShared sh;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = static_cast<int>(tc_uniform(tid >> 5)), lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&sh.ring.full[s], 1);
@@ -176,29 +191,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // -------------------------------------------------- issuer
             constexpr uint32_t ds = tc_idesc(BF16, kTileKeys, false), dv = tc_idesc(BF16, D, true);
             uint32_t place0 = 0, stays = 0, turns[2] = {0, 0};
+            const uint32_t leader = tc_elect(), tmem = tc_uniform(sh.tmem);
             PagedItem it;
             int kt0, kt1, out;
             while (walk.next(a, it, kt0, kt1, out)) {
                 const TileOrder order{it.r1 - it.r0 > 128, kt1 - kt0};
                 tile_wait(sh.ring, &sh.q_full, stays++);
                 auto scores = [&](int t, int j, bool last_use) {  // S_t = Q_t K_j^T
-                    const uint32_t p = place0 + order.key_at(j), s = p % kStages;
+                    const uint32_t p = place0 + order.key_at(j), s = tc_uniform(p % kStages);
                     tile_wait(sh.ring, &sh.ring.full[s], p / kStages);
                     tc_fence_after();
-                    if (lane == 0 && !sh.ring.abort) {
-                        const uint32_t q0 = smem_u32(sq) + (order.interleaved ? t * 128 * D * 2 : 0), k0 = smem_u32(ring) + s * kStage;
+                    const uint32_t go = tc_uniform(!sh.ring.abort) ? leader : 0u;
+                    const uint32_t q0 = tc_desc_rows(smem_u32(sq) + (order.interleaved ? t * 128 * D * 2 : 0));
+                    const uint32_t k0 = tc_desc_rows(smem_u32(ring) + s * kStage);
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint32_t at = (k >> 2) * 16384 + (k & 3) * 32;
-                            tc_mma_ss(tmem + t * 128, tc_desc_rows(q0 + at), tc_desc_rows(k0 + at), ds, k > 0);
-                        }
-                        tc_commit(&sh.s_full[t]);
-                        if (last_use) tc_commit(&sh.ring.empty[s]);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                        tc_mma_ss(tmem + t * 128, q0 + at, k0 + at, ds, k > 0, go);
                     }
-                    __syncwarp();
+                    tc_commit(&sh.s_full[t], go);
+                    if (last_use) tc_commit(&sh.ring.empty[s], go);
                 };
                 auto values = [&](int t, int j, bool first, bool last, bool first_use, bool last_use) {  // O_t += P_t V_j
-                    const uint32_t p = place0 + order.value_at(j), s = p % kStages;
+                    const uint32_t p = place0 + order.value_at(j), s = tc_uniform(p % kStages);
                     tile_wait(sh.ring, &sh.ring.full[s], p / kStages);
                     // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
                     const int key0 = (kt0 + j) * kTileKeys;
@@ -213,16 +228,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     tile_wait(sh.ring, &sh.p_full[t], turns[t]++);
                     tc_fence_after();
-                    if (lane == 0 && !sh.ring.abort) {
-                        const uint32_t v0 = smem_u32(ring) + s * kStage;
+                    const uint32_t go = tc_uniform(!sh.ring.abort) ? leader : 0u;
+                    const uint32_t v0 = tc_desc_cols(smem_u32(ring) + s * kStage);
 #pragma unroll
-                        for (int k = 0; k < kTileKeys / 16; ++k)
-                            tc_mma_ts(tmem + kO + t * 128, tmem + t * 128 + k * 8, tc_desc_cols(v0 + k * 2048), dv,
-                                      !(first && k == 0));
-                        if (last_use) tc_commit(&sh.ring.empty[s]);
-                        if (last) tc_commit(&sh.o_full[t]);
-                    }
-                    __syncwarp();
+                    for (int k = 0; k < kTileKeys / 16; ++k)
+                        tc_mma_ts(tmem + kO + t * 128, tmem + t * 128 + k * 8, v0 + k * (2048 >> 4), dv, k > 0 || !first, go);
+                    if (last_use) tc_commit(&sh.ring.empty[s], go);
+                    if (last) tc_commit(&sh.o_full[t], go);
                 };
                 const int n = order.n;
                 if (order.interleaved) {
@@ -245,11 +257,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 place0 += 2 * n;
             }
             // every product issued completes before TMEM is freed
-            if (lane == 0) {
-                tc_commit(&sh.drain);
-                mbar_wait_bounded(&sh.drain, 0, kTilePolls);
-            }
-            __syncwarp();
+            tc_commit(&sh.drain, leader);
+            mbar_wait_bounded(&sh.drain, 0, kTilePolls);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
