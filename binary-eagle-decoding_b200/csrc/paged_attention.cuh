@@ -383,9 +383,9 @@ __device__ __forceinline__ void paged_zero_rows(const PagedArgs &a) {
 // ------------------------------------------------------------------ tiles
 //
 // Both attention kernels read K and V in tiles of 128 keys of one kv head, D / 64
-// blocks of 128 rows of 64 values (128 bytes, 128-byte-swizzled), which one warp
-// loads by TMA, a lane to a box of one page piece and block, into a ring of stages
-// that the other warps release.
+// blocks of 128 rows of 64 values (128 bytes, 128-byte-swizzled), which the loading
+// warps fetch by TMA, a lane to a box of one page piece and block, into a ring of
+// stages that the other warps release.
 
 constexpr int kTileKeys = 128;
 constexpr int kRowsItem = 64;  // rows of an item: mma.sync kernel
@@ -405,10 +405,13 @@ struct TileRing {
 
 // Waits for phase `count` (0, 1, ..) of a barrier.  A wait that runs out sets `abort`,
 // after which all waits pass: every role walks to its end.
-__device__ __forceinline__ void tile_wait(TileRing &ring, uint64_t *b, uint32_t count) {
-    for (uint32_t i = 0; i < kTilePolls; ++i)
-        if (mbar_try_wait(b, count & 1) || ring.abort) return;
+__device__ __forceinline__ bool tile_wait(TileRing &ring, uint64_t *b, uint32_t count) {
+    for (uint32_t i = 0; i < kTilePolls; ++i) {
+        if (mbar_try_wait(b, count & 1)) return true;
+        if (ring.abort) return false;
+    }
     ring.abort = 1;
+    return false;
 }
 __device__ __forceinline__ void tile_arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
@@ -431,12 +434,14 @@ struct PagedMaps {
     int heads_outer;  // coordinates (column, slot, head, page), else (column, head, slot, page)
 };
 
-// The loading warp's whole run.  A piece without a key that some row sees, or on a page
+// The whole run of loading warp `turn` of LOADERS, which have the tiles in turn: a warp
+// issues the boxes of its lanes one after the other (about 130 cycles each), which at
+// pages of 16 keys is longer than a tile takes to arrive.  A piece without a key that some row sees, or on a page
 // outside the pool, is read as zeros (a box behind the last page).
-template <int D, int STAGES, typename Walk>
+template <int D, int STAGES, int LOADERS, typename Walk>
 __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileRing &ring, uint8_t *stages,
                                            const CUtensorMap *k_map, const CUtensorMap *v_map, int heads_outer,
-                                           int alternating_rows) {
+                                           int interleave_above, uint32_t turn) {
     const int lane = threadIdx.x & 31;
     asm volatile("fence.proxy.async.global;" ::: "memory");  // the cache rows that earlier kernels wrote
     const int piece = 1 << min(a.page_shift, 7);             // keys of a box
@@ -446,12 +451,13 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
     PagedItem it;
     int kt0, kt1, out;
     while (walk.next(a, it, kt0, kt1, out)) {
-        const TileOrder order{it.r1 - it.r0 > alternating_rows, kt1 - kt0};
+        const TileOrder order{it.r1 - it.r0 > interleave_above, kt1 - kt0};
         const int32_t *table = a.table + it.b * a.table_ld;
         int next_key = 0, next_value = 0;
         for (int i = 0; i < 2 * order.n; ++i, ++place) {
             const bool value = next_key == order.n || order.value_at(next_value) == i;
             const int kt = kt0 + (value ? next_value++ : next_key++);
+            if (place % LOADERS != turn) continue;
             const int key = kt * kTileKeys + part * piece;
             const bool seen = block < D / 64 && key < it.hi && key + piece > it.lo;
             int page = seen ? __ldg(table + (key >> a.page_shift)) : -1;
@@ -479,7 +485,7 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
     // after a wait ran out: the copies in flight land before the CTA ends
     if (ring.abort)
         for (uint32_t j = place > STAGES ? place - STAGES : 0; j < place; ++j)
-            mbar_wait_bounded(&ring.full[j % STAGES], (j / STAGES) & 1, kTilePolls);
+            if (j % LOADERS == turn) mbar_wait_bounded(&ring.full[j % STAGES], (j / STAGES) & 1, kTilePolls);
 }
 
 // ------------------------------------------------------------------ launches

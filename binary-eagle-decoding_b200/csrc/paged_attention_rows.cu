@@ -2,8 +2,8 @@
 // draft blocks, and fp32 rows of any count.  The mathematics and the work split are
 // those at the head of paged_attention.cu, with 64 rows to an item.
 //
-// One CTA per SM: a warp loads key and value tiles by TMA into a ring of six stages
-// (about 190 KB in flight, which is what covers HBM's latency), eight warps
+// One CTA per SM: four warps load key and value tiles by TMA into a ring of six
+// stages (about 190 KB in flight, which is what covers HBM's latency), eight warps
 // compute.  RW of them lie along the rows (16 each), 8 / RW along the keys of a
 // tile; each has the running maximum, sum and O of its rows over its keys, so the
 // warps meet only at the end of a stay.  S = Q K^T and O += P V are m16n8k16 MMAs.
@@ -16,7 +16,7 @@ namespace bd {
 
 constexpr int kRowsWarps = 8;
 constexpr int kRowsExtra = 1;  // a stay's Q, joining and output, in units
-constexpr int kRowsThreads = 384;  // the last three warps only lend their registers
+constexpr int kRowsThreads = 384;
 
 template <int D>
 constexpr int rows_stages() {
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
     if (warp >= kRowsWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == kRowsWarps) load_tiles<D, kStages>(a, walk, sh.ring, stages, &k_map, &v_map, heads_outer, -1);
+        load_tiles<D, kStages, 4>(a, walk, sh.ring, stages, &k_map, &v_map, heads_outer, -1, warp - kRowsWarps);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         uint32_t place = 0;

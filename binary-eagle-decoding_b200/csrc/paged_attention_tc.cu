@@ -3,18 +3,21 @@
 // joining of partials are those of paged_attention.cu, with 256 rows to an item and
 // 128 keys to a unit.
 //
-// One CTA per SM, 10 warps.  Two streams of work alternate on the tensor pipe so
-// that the softmax of one runs under the products of the other:
+// One CTA per SM.  Two streams of work alternate on the tensor pipe:
 //   * an item of more than 128 rows: stream t has rows [128 t, 128 t + 128), and both
 //     use every key tile, which is loaded once;
-//   * an item of up to 128 rows: both streams have the same rows, stream t takes every
-//     second key tile, and the two (maximum, sum, O) are joined at the end.
+//   * an item of up to 128 rows: both streams have the same rows, stream t takes keys
+//     [64 t, 64 t + 64) of every tile, and the two (maximum, sum, O) are joined at the
+//     end of the stay.
+// A stream goes by steps of 64 keys and has two buffers for S, so that its next S is
+// ready when the softmax of this one ends: with one buffer of 128 keys the chain S,
+// softmax, P V of a stream left the tensor pipe 55 % idle (8192 + 2048 keys: 681 us).
 // Warps 0-3 and 4-7 are the softmax of stream 0 and 1, a thread to a row: S from
 // TMEM, running maximum and sum, P as 16-bit values back over S's columns.  O stays
 // in TMEM; a row's O is rescaled only when its maximum has grown by more than 2^8
 // since the last time (P is at most 2^8 then, the sum and O scale alike), which
-// takes the rescaling off the usual path.  Warp 8 loads key and value tiles by TMA
-// (a box per page piece and 64 columns) into one ring in the order of their use;
+// takes the rescaling off the usual path.  Warps 8, 10 and 11 load key and value tiles by
+// TMA (a box per page piece and 64 columns) into one ring in the order of their use;
 // warp 9 issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM,
 // V as it lies, its rows being the reduction).
 //
@@ -24,7 +27,8 @@
 
 namespace bd {
 
-constexpr int kTcThreads = 384;  // warps 10 and 11 only lend their registers
+constexpr int kTcStep = 64;  // keys of a step of a stream
+constexpr int kTcThreads = 384;
 constexpr int kTcExtra = 3;       // a stay's Q, first and last products and output, in units
 constexpr float kTcSlack = 8.0f;  // growth of a maximum (log2) that leaves O as it is
 
@@ -39,7 +43,7 @@ constexpr size_t tc_smem() {
 
 struct TcShared {
     TileRing ring;
-    uint64_t q_full, s_full[2], p_full[2], o_full[2], drain;
+    uint64_t q_full, s_full[2][2], p_full[2][2], o_full[2], drain;  // of a stream, of its S buffers
     uint32_t tmem;
     float2 ml[128];
     PagedShared walk;
@@ -123,8 +127,18 @@ __device__ __forceinline__ uint32_t tc_elect() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
     return leader;
 }
-// A value that is the same in all lanes, as one the compiler knows to be.
-__device__ __forceinline__ uint32_t tc_uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// A value that is the same in all lanes, as one the compiler knows to be: a reduction
+// over the warp leaves its result in a uniform register.
+__device__ __forceinline__ uint32_t tc_uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
+// tile_wait() by a whole warp, in branches that are the same for all lanes.
+__device__ __forceinline__ bool tc_wait(TileRing &ring, uint64_t *b, uint32_t count) {
+    for (uint32_t i = 0; i < kTilePolls; ++i) {
+        if (__any_sync(0xffffffffu, mbar_try_wait(b, count & 1))) return true;
+        if (__any_sync(0xffffffffu, ring.abort)) return false;
+    }
+    ring.abort = 1;
+    return false;
+}
 
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float m;
@@ -142,13 +156,113 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// The issuing warp.  The tensor pipe has few MMAs queued, so what stands between them
+// counts: all that an MMA takes is warp-uniform to the compiler's eyes, and the
+// buffers, streams and halves are constants of the code (stepping through them with
+// variables: 815 instead of 682 us at 8192 + 2048 keys).
+template <int D, bool BF16>
+struct TcIssuer {
+    static constexpr int kStages = tc_stages<D>(), kStage = tile_bytes<D>();
+    static constexpr uint32_t kScores = tc_idesc(BF16, kTcStep, false), kValues = tc_idesc(BF16, D, true);
+    static constexpr uint32_t kHalf = kTcStep * 128 >> 4;  // of a tile, in descriptor units
+    TcShared &sh;
+    uint8_t *ring;
+    uint32_t columns, q_desc, k_desc, v_desc, go;
+    uint32_t p_phase[2] = {0, 0};       // of the S buffers
+    uint32_t next = 0, next_phase = 0;  // the ring's next tile, in the order of first use
+    uint32_t k_stage = 0, v_stage = 0;  // the tiles in use
+
+    __device__ __forceinline__ TcIssuer(TcShared &s, uint32_t q, uint8_t *r) : sh(s), ring(r) {
+        columns = tc_uniform(s.tmem);
+        q_desc = tc_desc_rows(q);
+        k_desc = tc_desc_rows(smem_u32(r));
+        v_desc = tc_desc_cols(smem_u32(r));
+        go = tc_elect();
+    }
+    __device__ __forceinline__ void wait(uint64_t *b, uint32_t count) {
+        if (!tc_wait(sh.ring, b, count)) go = 0;
+        tc_fence_after();
+    }
+    __device__ __forceinline__ void tile(uint32_t &stage) {
+        stage = next;
+        wait(&sh.ring.full[stage], next_phase);
+        next = next + 1 == kStages ? 0 : next + 1;
+        next_phase ^= next == 0;
+    }
+    // S_T = Q_T K^T over 64 keys, into buffer B
+    template <bool BOTH, int T, int B>
+    __device__ __forceinline__ void scores() {
+        constexpr uint32_t half = BOTH ? B : T;
+        if (T == 0 && (!BOTH || B == 0)) tile(k_stage);
+        const uint32_t q0 = q_desc + (BOTH ? T * (128 * D * 2 >> 4) : 0);
+        const uint32_t k0 = k_desc + k_stage * (kStage >> 4) + half * kHalf;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+            tc_mma_ss(columns + T * 128 + B * kTcStep, q0 + at, k0 + at, kScores, k > 0, go);
+        }
+        tc_commit(&sh.s_full[T][B], go);
+        if (T == 1 && (!BOTH || B == 1)) tc_commit(&sh.ring.empty[k_stage], go);
+    }
+    // O_T += P_T V over the 64 keys of buffer B
+    template <bool BOTH, int T, int B>
+    __device__ __forceinline__ void values(const PagedItem &it, int key0, uint32_t accumulate) {
+        constexpr uint32_t half = BOTH ? B : T;
+        if (T == 0 && (!BOTH || B == 0)) {
+            tile(v_stage);
+            // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
+            if (tc_uniform(key0 < it.lo || key0 + kTileKeys > it.hi)) {
+                for (int x = threadIdx.x & 31; x < kTileKeys * (D / 8); x += 32) {
+                    const int r = (x >> 3) & (kTileKeys - 1);
+                    if (key0 + r < it.lo || key0 + r >= it.hi)
+                        *reinterpret_cast<uint4 *>(ring + v_stage * kStage + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+        }
+        wait(&sh.p_full[T][B], p_phase[B]);
+        const uint32_t v0 = v_desc + v_stage * (kStage >> 4) + half * kHalf;
+#pragma unroll
+        for (int k = 0; k < kTcStep / 16; ++k)
+            tc_mma_ts(columns + 256 + T * 128, columns + T * 128 + B * kTcStep + k * 8, v0 + k * (2048 >> 4), kValues,
+                      k > 0 ? 1u : accumulate, go);
+        tc_commit(&sh.o_full[T], go);
+        if (T == 1 && (!BOTH || B == 1)) tc_commit(&sh.ring.empty[v_stage], go);
+    }
+    template <bool BOTH, int B>
+    __device__ __forceinline__ void step(const PagedItem &it, int key0, bool more, uint32_t accumulate) {
+        values<BOTH, 0, B>(it, key0, accumulate);
+        if (more) scores<BOTH, 0, B>();
+        values<BOTH, 1, B>(it, key0, accumulate);
+        if (more) scores<BOTH, 1, B>();
+        p_phase[B] ^= 1;
+    }
+    // The products of a stay of n key tiles.
+    template <bool BOTH>
+    __device__ __forceinline__ void stay(const PagedItem &it, int kt0, int n) {
+        const int steps = BOTH ? 2 * n : n;
+        scores<BOTH, 0, 0>();
+        scores<BOTH, 1, 0>();
+        if (steps > 1) {
+            scores<BOTH, 0, 1>();
+            scores<BOTH, 1, 1>();
+        }
+        int key0 = kt0 * kTileKeys;
+        for (int i = 0; i < steps; i += 2, key0 += BOTH ? kTileKeys : 2 * kTileKeys) {
+            step<BOTH, 0>(it, key0, i + 2 < steps, i > 0);
+            if (i + 1 < steps) step<BOTH, 1>(it, BOTH ? key0 : key0 + kTileKeys, i + 3 < steps, 1u);
+        }
+    }
+};
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_tc_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                     int heads_outer) {
     constexpr int MODE = BF16 ? PAGED_BF16 : PAGED_F16;
-    constexpr int kStages = tc_stages<D>(), kStage = tile_bytes<D>(), kBlocks = D / 64;
-    constexpr uint32_t kO = 256;  // TMEM columns: S0, S1 (P over them), O0, O1 at 256 and 384
+    constexpr int kStages = tc_stages<D>();
+    constexpr uint32_t kO = 256;  // TMEM columns: two S buffers of each stream (P over them), O at 256 and 384
     extern __shared__ uint8_t tc_raw[];
     uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = sq + 2 * 128 * D * 2;
@@ -161,8 +275,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         mbar_init(&sh.q_full, 8);
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&sh.s_full[t], 1);
-            mbar_init(&sh.p_full[t], 4);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh.s_full[t][i], 1);
+                mbar_init(&sh.p_full[t][i], 4);
+            }
             mbar_init(&sh.o_full[t], 1);
         }
         mbar_init(&sh.drain, 1);
@@ -182,100 +298,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     PagedWalk<kTcItem, kTileKeys, kTcExtra, true> walk;
     if (tid == 0) a.parts[1].open[blockIdx.x].last = -1;
     const bool any = walk.begin(a, sh.walk, blockIdx.x, gridDim.x);
-    // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
+    // registers: 384 x 168 at launch = 128 x 104 + 256 x 200
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (any && warp == 8) {
-            load_tiles<D, kStages>(a, walk, sh.ring, ring, &k_map, &v_map, heads_outer, 128);
-        } else if (any && warp == 9) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (any && warp != 9) {
+            load_tiles<D, kStages, 3>(a, walk, sh.ring, ring, &k_map, &v_map, heads_outer, 128, warp == 8 ? 0 : warp - 9);
+        } else if (any) {
             // -------------------------------------------------- issuer
-            constexpr uint32_t ds = tc_idesc(BF16, kTileKeys, false), dv = tc_idesc(BF16, D, true);
-            uint32_t place0 = 0, stays = 0, turns[2] = {0, 0};
-            const uint32_t leader = tc_elect(), tmem = tc_uniform(sh.tmem);
+            TcIssuer<D, BF16> issue(sh, smem_u32(sq), ring);
+            uint32_t stays = 0;
             PagedItem it;
             int kt0, kt1, out;
-            while (walk.next(a, it, kt0, kt1, out)) {
-                const TileOrder order{it.r1 - it.r0 > 128, kt1 - kt0};
-                tile_wait(sh.ring, &sh.q_full, stays++);
-                auto scores = [&](int t, int j, bool last_use) {  // S_t = Q_t K_j^T
-                    const uint32_t p = place0 + order.key_at(j), s = tc_uniform(p % kStages);
-                    tile_wait(sh.ring, &sh.ring.full[s], p / kStages);
-                    tc_fence_after();
-                    const uint32_t go = tc_uniform(!sh.ring.abort) ? leader : 0u;
-                    const uint32_t q0 = tc_desc_rows(smem_u32(sq) + (order.interleaved ? t * 128 * D * 2 : 0));
-                    const uint32_t k0 = tc_desc_rows(smem_u32(ring) + s * kStage);
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                        tc_mma_ss(tmem + t * 128, q0 + at, k0 + at, ds, k > 0, go);
-                    }
-                    tc_commit(&sh.s_full[t], go);
-                    if (last_use) tc_commit(&sh.ring.empty[s], go);
-                };
-                auto values = [&](int t, int j, bool first, bool last, bool first_use, bool last_use) {  // O_t += P_t V_j
-                    const uint32_t p = place0 + order.value_at(j), s = tc_uniform(p % kStages);
-                    tile_wait(sh.ring, &sh.ring.full[s], p / kStages);
-                    // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
-                    const int key0 = (kt0 + j) * kTileKeys;
-                    if (first_use && (key0 < it.lo || key0 + kTileKeys > it.hi)) {
-                        for (int i = lane; i < kTileKeys * kBlocks * 8; i += 32) {
-                            const int r = (i >> 3) & (kTileKeys - 1);
-                            if (key0 + r < it.lo || key0 + r >= it.hi)
-                                *reinterpret_cast<uint4 *>(ring + s * kStage + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    tile_wait(sh.ring, &sh.p_full[t], turns[t]++);
-                    tc_fence_after();
-                    const uint32_t go = tc_uniform(!sh.ring.abort) ? leader : 0u;
-                    const uint32_t v0 = tc_desc_cols(smem_u32(ring) + s * kStage);
-#pragma unroll
-                    for (int k = 0; k < kTileKeys / 16; ++k)
-                        tc_mma_ts(tmem + kO + t * 128, tmem + t * 128 + k * 8, v0 + k * (2048 >> 4), dv, k > 0 || !first, go);
-                    if (last_use) tc_commit(&sh.ring.empty[s], go);
-                    if (last) tc_commit(&sh.o_full[t], go);
-                };
-                const int n = order.n;
-                if (order.interleaved) {
-                    scores(0, 0, false);
-                    scores(1, 0, true);
-                    for (int j = 0; j < n; ++j) {
-                        values(0, j, j == 0, j + 1 == n, true, false);
-                        if (j + 1 < n) scores(0, j + 1, false);
-                        values(1, j, j == 0, j + 1 == n, false, true);
-                        if (j + 1 < n) scores(1, j + 1, true);
-                    }
-                } else {
-                    scores(0, 0, true);
-                    if (n > 1) scores(1, 1, true);
-                    for (int j = 0; j < n; ++j) {
-                        values(j & 1, j, j < 2, j + 2 >= n, true, true);
-                        if (j + 2 < n) scores(j & 1, j + 2, true);
-                    }
-                }
-                place0 += 2 * n;
+            while (tc_uniform(walk.next(a, it, kt0, kt1, out))) {
+                issue.wait(&sh.q_full, stays++);
+                if (tc_uniform(it.r1 - it.r0 > 128))
+                    issue.template stay<true>(it, kt0, tc_uniform(kt1 - kt0));
+                else
+                    issue.template stay<false>(it, kt0, tc_uniform(kt1 - kt0));
             }
             // every product issued completes before TMEM is freed
-            tc_commit(&sh.drain, leader);
+            tc_commit(&sh.drain, tc_elect());
             mbar_wait_bounded(&sh.drain, 0, kTilePolls);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // -------------------------------------------------- softmax: a thread to a row
         const int t = warp >> 2, wrow = (warp & 3) * 32, lrow = wrow + lane;
-        const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16);
-        const uint32_t o_at = s_at - t * 128 + kO + t * 128;
+        const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16), o_at = s_at + kO;
         const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-        uint32_t tiles_seen = 0, ends[2] = {0, 0};
+        uint32_t steps[2] = {0, 0}, products = 0, other = 0;  // through each S buffer, into O, into the other stream's O
         PagedItem it;
         int kt0, kt1, out;
         while (any && walk.next(a, it, kt0, kt1, out)) {
             const int n = kt1 - kt0, rows = it.r1 - it.r0;
             if (tid == 0 && out >= 0 && (out & 1)) a.parts[1].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
             const bool both = rows > 128;
-            const int mine = both ? n : (n - t + 1) / 2;  // key tiles of this stream
+            const int count = both ? 2 * n : n;  // steps of 64 keys
             const int row = it.r0 + (both ? t * 128 : 0) + lrow;
             const bool live = row < it.r1;
             const bool warp_live = row - lane < it.r1;
@@ -307,99 +366,99 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0) tile_arrive(&sh.q_full);
 
             float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < mine; ++j) {
-                tile_wait(sh.ring, &sh.s_full[t], tiles_seen++);
+            for (int i = 0; i < count; ++i) {
+                const int buffer = i & 1;
+                const uint32_t at = s_at + buffer * kTcStep;
+                tile_wait(sh.ring, &sh.s_full[t][buffer], steps[buffer]++);
                 tc_fence_after();
                 if (warp_live) {
-                    const int key0 = (kt0 + (both ? j : 2 * j + t)) * kTileKeys;
-                    float s[4][32];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tc_ld32(s_at + 32 * i, s[i]);
+                    const int key0 = both ? (kt0 * 2 + i) * kTcStep : (kt0 + i) * kTileKeys + t * kTcStep;
+                    float s[2][32];
+                    tc_ld32(at, s[0]);
+                    tc_ld32(at + 32, s[1]);
                     tc_ld_wait();
-                    if (key0 < it.lo_all || key0 + kTileKeys > it.hi_all) {
+                    if (key0 < it.lo_all || key0 + kTcStep > it.hi_all) {
                         const int first = lo - key0, last = hi - key0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int x = 0; x < 2; ++x)
 #pragma unroll
                             for (int k = 0; k < 32; ++k)
-                                if (32 * i + k < first || 32 * i + k >= last) s[i][k] = -INFINITY;
+                                if (32 * x + k < first || 32 * x + k >= last) s[x][k] = -INFINITY;
                     }
                     float top[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        top[i] = fmaxf(s[i][0], s[i][1]);
+                    for (int x = 0; x < 4; ++x) {
+                        const float *v = &s[x >> 1][(x & 1) * 16];
+                        top[x] = fmaxf(v[0], v[1]);
 #pragma unroll
-                        for (int k = 2; k < 32; k += 2) top[i] = max3(top[i], s[i][k], s[i][k + 1]);
+                        for (int k = 2; k < 16; k += 2) top[x] = max3(top[x], v[k], v[k + 1]);
                     }
-                    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                    const float now = fmaxf(max3(top[0], top[1], top[2]), top[3]) * c;
                     const bool grows = now > m + kTcSlack || m == -INFINITY;
                     if (__any_sync(0xffffffffu, grows && m != -INFINITY)) {
-                        // S_t of this tile being complete, so is every earlier product of the stream
+                        // the products so far are in O (this S says so of all but the last)
+                        tile_wait(sh.ring, &sh.o_full[t], products - 1);
+                        tc_fence_after();
                         const float back = grows ? exp2_fast(m - now) : 1.0f;
                         l *= m == -INFINITY ? 1.0f : back;
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
+                        for (int x = 0; x < D / 32; ++x) {
                             float o[32];
                             uint32_t w[32];
-                            tc_ld32(o_at + 32 * i, o);
+                            tc_ld32(o_at + 32 * x, o);
                             tc_ld_wait();
 #pragma unroll
                             for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(m == -INFINITY ? 0.0f : o[k] * back);
-                            tc_st32(o_at + 32 * i, w);
+                            tc_st32(o_at + 32 * x, w);
                         }
                     }
                     if (grows) m = now;
                     const float base = m == -INFINITY ? 0.0f : m;
                     const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
                     float2 sum[4];
+                    uint32_t w[32];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.0f, 0.0f);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const float *x = &s[2 * i + (k >> 4)][2 * (k & 15)];
-                            float2 p = __ffma2_rn(make_float2(x[0], x[1]), c2, base2);
-                            p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
-                            sum[k & 3] = __fadd2_rn(sum[k & 3], p);
-                            w[k] = tc_pack<BF16>(p.x, p.y);
-                        }
-                        tc_st32(s_at + 32 * i, w);
+                    for (int k = 0; k < 32; ++k) {
+                        const float *x = &s[k >> 4][2 * (k & 15)];
+                        float2 p = __ffma2_rn(make_float2(x[0], x[1]), c2, base2);
+                        p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
+                        sum[k & 3] = k < 4 ? p : __fadd2_rn(sum[k & 3], p);
+                        w[k] = tc_pack<BF16>(p.x, p.y);
                     }
+                    tc_st32(at, w);
                     const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
                     l += all.x + all.y;
                     tc_st_wait();
                 }
+                ++products;
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tile_arrive(&sh.p_full[t]);
+                if (lane == 0) tile_arrive(&sh.p_full[t][buffer]);
             }
-            // the end of the stay: this stream's products, and with the same rows the other's too
-            if (both || t == 0 || mine > 0) tile_wait(sh.ring, &sh.o_full[t], ends[t]);
-            if (!both && t == 1) tile_wait(sh.ring, &sh.o_full[0], ends[0]);
-            if (!both && t == 0 && n > 1) tile_wait(sh.ring, &sh.o_full[1], ends[1]);
-            ++ends[0];
-            ends[1] += both || n > 1;
+            // the end of the stay: this stream's products (its last S says that all but two are
+            // done; a barrier tells two phases apart), and with the same rows the other's too
+            if (count > 1) tile_wait(sh.ring, &sh.o_full[t], products - 2);
+            tile_wait(sh.ring, &sh.o_full[t], products - 1);
+            if (!both) tile_wait(sh.ring, &sh.o_full[t ^ 1], other + n - 1);
+            other += count;
             tc_fence_after();
             float4 *swap = reinterpret_cast<float4 *>(sq);  // Q is done with: O of stream 1, [column / 4][row]
             float mine_w = 1.0f, other_w = 0.0f;
             if (!both) {
                 if (t == 1 && warp_live) {
                     sh.ml[lrow] = make_float2(m, l);
-                    if (mine > 0)
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
-                            float o[32];
-                            tc_ld32(o_at + 32 * i, o);
-                            tc_ld_wait();
+                    for (int i = 0; i < D / 32; ++i) {
+                        float o[32];
+                        tc_ld32(o_at + 32 * i, o);
+                        tc_ld_wait();
 #pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                swap[(i * 8 + k) * 128 + lrow] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                        }
+                        for (int k = 0; k < 8; ++k)
+                            swap[(i * 8 + k) * 128 + lrow] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    }
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (t == 0 && warp_live && n > 1) {
+                if (t == 0 && warp_live) {
                     const float2 x = sh.ml[lrow];
                     const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
                     mine_w = exp2_fast(m - base);
@@ -418,7 +477,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     float o[32];
                     tc_ld32(o_at + 32 * i, o);
                     tc_ld_wait();
-                    if (!both && n > 1) {
+                    if (!both) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const float4 x = swap[(i * 8 + k) * 128 + lrow];
