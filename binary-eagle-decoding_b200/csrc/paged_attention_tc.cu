@@ -16,10 +16,10 @@
 // TMEM, running maximum and sum, P as 16-bit values back over S's columns.  O stays
 // in TMEM; a row's O is rescaled only when its maximum has grown by more than 2^8
 // since the last time (P is at most 2^8 then, the sum and O scale alike), which
-// takes the rescaling off the usual path.  Warps 8, 10 and 11 load key and value tiles by
-// TMA (a box per page piece and 64 columns) into one ring in the order of their use;
-// warp 9 issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM,
-// V as it lies, its rows being the reduction).
+// takes the rescaling off the usual path.  Warps 10 and 11 load key and value tiles by TMA
+// (a box per page piece and 64 columns) into one ring in the order of their use;
+// warps 8 and 9 issue, each for a stream, S = Q K^T (both operands in shared memory)
+// and O += P V (P in TMEM, V as it lies, its rows being the reduction).
 //
 // Every wait is bounded; one that runs out sets BD_FLAG_TIMEOUT and turns the waits
 // that follow into passes, so that all roles walk to their end.
@@ -43,7 +43,9 @@ constexpr size_t tc_smem() {
 
 struct TcShared {
     TileRing ring;
-    uint64_t q_full, s_full[2][2], p_full[2][2], o_full[2], drain;  // of a stream, of its S buffers
+    // of a stream and of its S buffers.  A barrier's wait tells two phases apart, no more:
+    // o_step is for the products of a step, o_full for those of a stay.
+    uint64_t q_full, s_full[2][2], p_full[2][2], o_step[2][2], o_full[2], drain[2];
     uint32_t tmem;
     float2 ml[128];
     PagedShared walk;
@@ -156,11 +158,12 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// The issuing warp.  The tensor pipe has few MMAs queued, so what stands between them
-// counts: all that an MMA takes is warp-uniform to the compiler's eyes, and the
-// buffers, streams and halves are constants of the code (stepping through them with
-// variables: 815 instead of 682 us at 8192 + 2048 keys).
-template <int D, bool BF16>
+// The issuing warp of stream T.  A warp of its own for each stream: between two groups of
+// MMAs stand waits and commits of some 600 cycles, more than the tensor pipe has
+// queued, which the other stream's MMAs fill (one warp for both: 712 us at 8192 + 2048
+// keys).  All that an MMA takes is warp-uniform to the compiler's eyes, and buffers
+// and halves are constants of the code.
+template <int D, bool BF16, int T>
 struct TcIssuer {
     static constexpr int kStages = tc_stages<D>(), kStage = tile_bytes<D>();
     static constexpr uint32_t kScores = tc_idesc(BF16, kTcStep, false), kValues = tc_idesc(BF16, D, true);
@@ -189,11 +192,11 @@ struct TcIssuer {
         next = next + 1 == kStages ? 0 : next + 1;
         next_phase ^= next == 0;
     }
-    // S_T = Q_T K^T over 64 keys, into buffer B
-    template <bool BOTH, int T, int B>
+    // S = Q K^T over 64 keys, into buffer B
+    template <bool BOTH, int B>
     __device__ __forceinline__ void scores() {
         constexpr uint32_t half = BOTH ? B : T;
-        if (T == 0 && (!BOTH || B == 0)) tile(k_stage);
+        if (!BOTH || B == 0) tile(k_stage);
         const uint32_t q0 = q_desc + (BOTH ? T * (128 * D * 2 >> 4) : 0);
         const uint32_t k0 = k_desc + k_stage * (kStage >> 4) + half * kHalf;
 #pragma unroll
@@ -202,15 +205,16 @@ struct TcIssuer {
             tc_mma_ss(columns + T * 128 + B * kTcStep, q0 + at, k0 + at, kScores, k > 0, go);
         }
         tc_commit(&sh.s_full[T][B], go);
-        if (T == 1 && (!BOTH || B == 1)) tc_commit(&sh.ring.empty[k_stage], go);
+        if (!BOTH || B == 1) tc_commit(&sh.ring.empty[k_stage], go);
     }
-    // O_T += P_T V over the 64 keys of buffer B
-    template <bool BOTH, int T, int B>
+    // O += P V over the 64 keys of buffer B
+    template <bool BOTH, int B>
     __device__ __forceinline__ void values(const PagedItem &it, int key0, uint32_t accumulate) {
         constexpr uint32_t half = BOTH ? B : T;
-        if (T == 0 && (!BOTH || B == 0)) {
+        if (!BOTH || B == 0) {
             tile(v_stage);
             // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
+            // (both streams' warps write them, each before its own products)
             if (tc_uniform(key0 < it.lo || key0 + kTileKeys > it.hi)) {
                 for (int x = threadIdx.x & 31; x < kTileKeys * (D / 8); x += 32) {
                     const int r = (x >> 3) & (kTileKeys - 1);
@@ -227,32 +231,42 @@ struct TcIssuer {
         for (int k = 0; k < kTcStep / 16; ++k)
             tc_mma_ts(columns + 256 + T * 128, columns + T * 128 + B * kTcStep + k * 8, v0 + k * (2048 >> 4), kValues,
                       k > 0 ? 1u : accumulate, go);
-        tc_commit(&sh.o_full[T], go);
-        if (T == 1 && (!BOTH || B == 1)) tc_commit(&sh.ring.empty[v_stage], go);
-    }
-    template <bool BOTH, int B>
-    __device__ __forceinline__ void step(const PagedItem &it, int key0, bool more, uint32_t accumulate) {
-        values<BOTH, 0, B>(it, key0, accumulate);
-        if (more) scores<BOTH, 0, B>();
-        values<BOTH, 1, B>(it, key0, accumulate);
-        if (more) scores<BOTH, 1, B>();
+        tc_commit(&sh.o_step[T][B], go);
+        if (!BOTH || B == 1) tc_commit(&sh.ring.empty[v_stage], go);
         p_phase[B] ^= 1;
     }
     // The products of a stay of n key tiles.
     template <bool BOTH>
     __device__ __forceinline__ void stay(const PagedItem &it, int kt0, int n) {
         const int steps = BOTH ? 2 * n : n;
-        scores<BOTH, 0, 0>();
-        scores<BOTH, 1, 0>();
-        if (steps > 1) {
-            scores<BOTH, 0, 1>();
-            scores<BOTH, 1, 1>();
-        }
+        scores<BOTH, 0>();
+        if (steps > 1) scores<BOTH, 1>();
         int key0 = kt0 * kTileKeys;
         for (int i = 0; i < steps; i += 2, key0 += BOTH ? kTileKeys : 2 * kTileKeys) {
-            step<BOTH, 0>(it, key0, i + 2 < steps, i > 0);
-            if (i + 1 < steps) step<BOTH, 1>(it, BOTH ? key0 : key0 + kTileKeys, i + 3 < steps, 1u);
+            values<BOTH, 0>(it, key0, i > 0);
+            if (i + 2 < steps) scores<BOTH, 0>();
+            if (i + 1 < steps) {
+                values<BOTH, 1>(it, BOTH ? key0 : key0 + kTileKeys, 1u);
+                if (i + 3 < steps) scores<BOTH, 1>();
+            }
         }
+        tc_commit(&sh.o_full[T], go);
+    }
+    template <typename Walk>
+    __device__ __forceinline__ void run(const PagedArgs &a, Walk &walk) {
+        uint32_t stays = 0;
+        PagedItem it;
+        int kt0, kt1, out;
+        while (tc_uniform(walk.next(a, it, kt0, kt1, out))) {
+            wait(&sh.q_full, stays++);
+            if (tc_uniform(it.r1 - it.r0 > 128))
+                stay<true>(it, kt0, tc_uniform(kt1 - kt0));
+            else
+                stay<false>(it, kt0, tc_uniform(kt1 - kt0));
+        }
+        // every product issued completes before TMEM is freed
+        tc_commit(&sh.drain[T], tc_elect());
+        mbar_wait_bounded(&sh.drain[T], 0, kTilePolls);
     }
 };
 
@@ -271,17 +285,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&sh.ring.full[s], 1);
-            mbar_init(&sh.ring.empty[s], 1);
+            mbar_init(&sh.ring.empty[s], 2);
         }
         mbar_init(&sh.q_full, 8);
         for (int t = 0; t < 2; ++t) {
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh.s_full[t][i], 1);
                 mbar_init(&sh.p_full[t][i], 4);
+                mbar_init(&sh.o_step[t][i], 1);
             }
             mbar_init(&sh.o_full[t], 1);
+            mbar_init(&sh.drain[t], 1);
         }
-        mbar_init(&sh.drain, 1);
         sh.ring.abort = 0;
         mbar_init_fence();
     }
@@ -301,25 +316,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // registers: 384 x 168 at launch = 128 x 104 + 256 x 200
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (any && warp != 9) {
-            load_tiles<D, kStages, 3>(a, walk, sh.ring, ring, &k_map, &v_map, heads_outer, 128, warp == 8 ? 0 : warp - 9);
-        } else if (any) {
-            // -------------------------------------------------- issuer
-            TcIssuer<D, BF16> issue(sh, smem_u32(sq), ring);
-            uint32_t stays = 0;
-            PagedItem it;
-            int kt0, kt1, out;
-            while (tc_uniform(walk.next(a, it, kt0, kt1, out))) {
-                issue.wait(&sh.q_full, stays++);
-                if (tc_uniform(it.r1 - it.r0 > 128))
-                    issue.template stay<true>(it, kt0, tc_uniform(kt1 - kt0));
-                else
-                    issue.template stay<false>(it, kt0, tc_uniform(kt1 - kt0));
-            }
-            // every product issued completes before TMEM is freed
-            tc_commit(&sh.drain, tc_elect());
-            mbar_wait_bounded(&sh.drain, 0, kTilePolls);
-        }
+        if (any && warp == 8)
+            TcIssuer<D, BF16, 0>(sh, smem_u32(sq), ring).run(a, walk);
+        else if (any && warp == 9)
+            TcIssuer<D, BF16, 1>(sh, smem_u32(sq), ring).run(a, walk);
+        else if (any)
+            load_tiles<D, kStages, 2>(a, walk, sh.ring, ring, &k_map, &v_map, heads_outer, 128, warp - 10);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // -------------------------------------------------- softmax: a thread to a row
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16), o_at = s_at + kO;
         const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-        uint32_t steps[2] = {0, 0}, products = 0, other = 0;  // through each S buffer, into O, into the other stream's O
+        uint32_t steps[2] = {0, 0}, stays = 0;  // steps: through each S buffer
         PagedItem it;
         int kt0, kt1, out;
         while (any && walk.next(a, it, kt0, kt1, out)) {
@@ -396,8 +398,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const float now = fmaxf(max3(top[0], top[1], top[2]), top[3]) * c;
                     const bool grows = now > m + kTcSlack || m == -INFINITY;
                     if (__any_sync(0xffffffffu, grows && m != -INFINITY)) {
-                        // the products so far are in O (this S says so of all but the last)
-                        tile_wait(sh.ring, &sh.o_full[t], products - 1);
+                        // the products so far are in O (this S says so of all but the last step's)
+                        tile_wait(sh.ring, &sh.o_step[t][buffer ^ 1], steps[buffer ^ 1] - 1);
                         tc_fence_after();
                         const float back = grows ? exp2_fast(m - now) : 1.0f;
                         l *= m == -INFINITY ? 1.0f : back;
@@ -430,21 +432,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     l += all.x + all.y;
                     tc_st_wait();
                 }
-                ++products;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tile_arrive(&sh.p_full[t][buffer]);
             }
-            // the end of the stay: this stream's products (its last S says that all but two are
-            // done; a barrier tells two phases apart), and with the same rows the other's too
-            if (count > 1) tile_wait(sh.ring, &sh.o_full[t], products - 2);
-            tile_wait(sh.ring, &sh.o_full[t], products - 1);
-            if (!both) tile_wait(sh.ring, &sh.o_full[t ^ 1], other + n - 1);
-            other += count;
+            tile_wait(sh.ring, &sh.o_full[t], stays++);
             tc_fence_after();
             float4 *swap = reinterpret_cast<float4 *>(sq);  // Q is done with: O of stream 1, [column / 4][row]
             float mine_w = 1.0f, other_w = 0.0f;
             if (!both) {
+                asm volatile("bar.sync 1, 256;" ::: "memory");  // neither stream reads Q any more
                 if (t == 1 && warp_live) {
                     sh.ml[lrow] = make_float2(m, l);
 #pragma unroll
