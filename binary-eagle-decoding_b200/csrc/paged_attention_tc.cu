@@ -87,6 +87,25 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) 
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// 16 columns, for the loops beside the main one (rolled: their code is fetched anew at
+// every stay).
+__device__ __forceinline__ void tc_ld16(uint32_t addr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const float (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+}
 __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -403,15 +422,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tc_fence_after();
                         const float back = grows ? exp2_fast(m - now) : 1.0f;
                         l *= m == -INFINITY ? 1.0f : back;
-#pragma unroll
-                        for (int x = 0; x < D / 32; ++x) {
-                            float o[32];
-                            uint32_t w[32];
-                            tc_ld32(o_at + 32 * x, o);
+#pragma unroll 1
+                        for (int x = 0; x < D / 16; ++x) {
+                            float o[16];
+                            tc_ld16(o_at + 16 * x, o);
                             tc_ld_wait();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(m == -INFINITY ? 0.0f : o[k] * back);
-                            tc_st32(o_at + 32 * x, w);
+                            for (int k = 0; k < 16; ++k) o[k] = m == -INFINITY ? 0.0f : o[k] * back;
+                            tc_st16(o_at + 16 * x, o);
                         }
                     }
                     if (grows) m = now;
@@ -444,15 +462,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 asm volatile("bar.sync 1, 256;" ::: "memory");  // neither stream reads Q any more
                 if (t == 1 && warp_live) {
                     sh.ml[lrow] = make_float2(m, l);
+#pragma unroll 1
+                    for (int i = 0; i < D / 16; ++i) {
+                            float o[16];
+                            tc_ld16(o_at + 16 * i, o);
+                            tc_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        float o[32];
-                        tc_ld32(o_at + 32 * i, o);
-                        tc_ld_wait();
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            swap[(i * 8 + k) * 128 + lrow] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                    }
+                            for (int k = 0; k < 4; ++k)
+                                swap[(i * 4 + k) * 128 + lrow] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        }
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (t == 0 && warp_live) {
@@ -469,15 +487,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float probe = 0.0f;
                 float *po = a.parts[1].o + (static_cast<int64_t>(max(out, 0)) * kTcItem + row - it.r0) * D;
                 const int64_t at = live ? paged_row_offset(a, it, row, a.out_row, D) : 0;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    float o[32];
-                    tc_ld32(o_at + 32 * i, o);
+#pragma unroll 1
+                for (int i = 0; i < D / 16; ++i) {
+                    float o[16];
+                    tc_ld16(o_at + 16 * i, o);
                     tc_ld_wait();
                     if (!both) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float4 x = swap[(i * 8 + k) * 128 + lrow];
+                        for (int k = 0; k < 4; ++k) {
+                            const float4 x = swap[(i * 4 + k) * 128 + lrow];
                             o[4 * k] = o[4 * k] * mine_w + x.x * other_w;
                             o[4 * k + 1] = o[4 * k + 1] * mine_w + x.y * other_w;
                             o[4 * k + 2] = o[4 * k + 2] * mine_w + x.z * other_w;
@@ -487,20 +505,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (out >= 0) {
                         if (live)
 #pragma unroll
-                            for (int k = 0; k < 32; k += 4)
-                                *reinterpret_cast<float4 *>(po + 32 * i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                            for (int k = 0; k < 16; k += 4)
+                                *reinterpret_cast<float4 *>(po + 16 * i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     } else {
-                        uint32_t w[16];
+                        uint32_t w[8];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
+                        for (int k = 0; k < 8; ++k) {
                             const float x = o[2 * k] * inv, y = o[2 * k + 1] * inv;
                             probe += 0.0f * x + 0.0f * y;
                             w[k] = tc_pack<BF16>(x, y);
                         }
                         if (live)
 #pragma unroll
-                            for (int k = 0; k < 16; k += 4)
-                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at + 32 * i + 2 * k) =
+                            for (int k = 0; k < 8; k += 4)
+                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at + 16 * i + 2 * k) =
                                     make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
                     }
                     __syncwarp();
