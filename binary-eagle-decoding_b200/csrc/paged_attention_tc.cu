@@ -177,25 +177,28 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// The issuing warp of stream T.  A warp of its own for each stream: between two groups of
+// The issuing warp of stream t.  A warp of its own for each stream: between two groups of
 // MMAs stand waits and commits of some 600 cycles, more than the tensor pipe has
-// queued, which the other stream's MMAs fill (one warp for both: 712 us at 8192 + 2048
-// keys).  All that an MMA takes is warp-uniform to the compiler's eyes, and buffers
-// and halves are constants of the code.
-template <int D, bool BF16, int T>
+// queued, which the other stream's MMAs fill.  All that an MMA takes is warp-uniform to
+// the compiler's eyes (moving operands to uniform registers took longer than the
+// MMAs), and each product stands once in the code, which all roles together must
+// keep small: a stay's own code is fetched anew after every main loop.
+template <int D, bool BF16>
 struct TcIssuer {
     static constexpr int kStages = tc_stages<D>(), kStage = tile_bytes<D>();
     static constexpr uint32_t kScores = tc_idesc(BF16, kTcStep, false), kValues = tc_idesc(BF16, D, true);
     static constexpr uint32_t kHalf = kTcStep * 128 >> 4;  // of a tile, in descriptor units
     TcShared &sh;
     uint8_t *ring;
-    uint32_t columns, q_desc, k_desc, v_desc, go;
-    uint32_t p_phase[2] = {0, 0};       // of the S buffers
+    const uint32_t t;
+    uint32_t s_columns, o_columns, q_desc, k_desc, v_desc, go;
+    uint32_t p_phase = 0;               // bit b: of S buffer b
     uint32_t next = 0, next_phase = 0;  // the ring's next tile, in the order of first use
     uint32_t k_stage = 0, v_stage = 0;  // the tiles in use
 
-    __device__ __forceinline__ TcIssuer(TcShared &s, uint32_t q, uint8_t *r) : sh(s), ring(r) {
-        columns = tc_uniform(s.tmem);
+    __device__ __forceinline__ TcIssuer(TcShared &s, uint32_t q, uint8_t *r, uint32_t stream) : sh(s), ring(r), t(stream) {
+        s_columns = tc_uniform(s.tmem) + t * 128;
+        o_columns = s_columns + 256;
         q_desc = tc_desc_rows(q);
         k_desc = tc_desc_rows(smem_u32(r));
         v_desc = tc_desc_cols(smem_u32(r));
@@ -211,65 +214,54 @@ struct TcIssuer {
         next = next + 1 == kStages ? 0 : next + 1;
         next_phase ^= next == 0;
     }
-    // S = Q K^T over 64 keys, into buffer B
-    template <bool BOTH, int B>
-    __device__ __forceinline__ void scores() {
-        constexpr uint32_t half = BOTH ? B : T;
-        if (!BOTH || B == 0) tile(k_stage);
-        const uint32_t q0 = q_desc + (BOTH ? T * (128 * D * 2 >> 4) : 0);
-        const uint32_t k0 = k_desc + k_stage * (kStage >> 4) + half * kHalf;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-            tc_mma_ss(columns + T * 128 + B * kTcStep, q0 + at, k0 + at, kScores, k > 0, go);
-        }
-        tc_commit(&sh.s_full[T][B], go);
-        if (!BOTH || B == 1) tc_commit(&sh.ring.empty[k_stage], go);
-    }
-    // O += P V over the 64 keys of buffer B
-    template <bool BOTH, int B>
-    __device__ __forceinline__ void values(const PagedItem &it, int key0, uint32_t accumulate) {
-        constexpr uint32_t half = BOTH ? B : T;
-        if (!BOTH || B == 0) {
-            tile(v_stage);
-            // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
-            // (both streams' warps write them, each before its own products)
-            if (tc_uniform(key0 < it.lo || key0 + kTileKeys > it.hi)) {
-                for (int x = threadIdx.x & 31; x < kTileKeys * (D / 8); x += 32) {
-                    const int r = (x >> 3) & (kTileKeys - 1);
-                    if (key0 + r < it.lo || key0 + r >= it.hi)
-                        *reinterpret_cast<uint4 *>(ring + v_stage * kStage + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+    // The products of a stay of n key tiles: before O += P V of step i, whose 64 keys are half
+    // i & 1 of a tile, or with the same rows in both streams half t of tile i, stands S = Q K^T
+    // of steps i and i + 1.
+    __device__ __forceinline__ void stay(const PagedItem &it, int kt0, int n, bool both) {
+        const int steps = both ? 2 * n : n;
+        const uint32_t q0 = q_desc + (both ? t * (128 * D * 2 >> 4) : 0);
+#pragma unroll 1
+        for (int i = -2; i < steps; ++i) {
+            const uint32_t b = i & 1, half = both ? b : t;
+            const bool first = !both || b == 0, last = !both || b == 1;  // use of a tile
+            if (i >= 0) {
+                if (first) {
+                    tile(v_stage);
+                    // rows of keys that no row sees may hold anything: zeros, so that 0 x row stays 0
+                    // (both streams' warps write them, each before its own products)
+                    const int key0 = (kt0 + (both ? i >> 1 : i)) * kTileKeys;
+                    if (tc_uniform(key0 < it.lo || key0 + kTileKeys > it.hi)) {
+                        for (int x = threadIdx.x & 31; x < kTileKeys * (D / 8); x += 32) {
+                            const int r = (x >> 3) & (kTileKeys - 1);
+                            if (key0 + r < it.lo || key0 + r >= it.hi)
+                                *reinterpret_cast<uint4 *>(ring + v_stage * kStage + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
-        }
-        wait(&sh.p_full[T][B], p_phase[B]);
-        const uint32_t v0 = v_desc + v_stage * (kStage >> 4) + half * kHalf;
+                wait(&sh.p_full[t][b], p_phase >> b);
+                const uint32_t v0 = v_desc + v_stage * (kStage >> 4) + half * kHalf, from = s_columns + b * kTcStep;
 #pragma unroll
-        for (int k = 0; k < kTcStep / 16; ++k)
-            tc_mma_ts(columns + 256 + T * 128, columns + T * 128 + B * kTcStep + k * 8, v0 + k * (2048 >> 4), kValues,
-                      k > 0 ? 1u : accumulate, go);
-        tc_commit(&sh.o_step[T][B], go);
-        if (!BOTH || B == 1) tc_commit(&sh.ring.empty[v_stage], go);
-        p_phase[B] ^= 1;
-    }
-    // The products of a stay of n key tiles.
-    template <bool BOTH>
-    __device__ __forceinline__ void stay(const PagedItem &it, int kt0, int n) {
-        const int steps = BOTH ? 2 * n : n;
-        scores<BOTH, 0>();
-        if (steps > 1) scores<BOTH, 1>();
-        int key0 = kt0 * kTileKeys;
-        for (int i = 0; i < steps; i += 2, key0 += BOTH ? kTileKeys : 2 * kTileKeys) {
-            values<BOTH, 0>(it, key0, i > 0);
-            if (i + 2 < steps) scores<BOTH, 0>();
-            if (i + 1 < steps) {
-                values<BOTH, 1>(it, BOTH ? key0 : key0 + kTileKeys, 1u);
-                if (i + 3 < steps) scores<BOTH, 1>();
+                for (int k = 0; k < kTcStep / 16; ++k)
+                    tc_mma_ts(o_columns, from + k * 8, v0 + k * (2048 >> 4), kValues, k > 0 ? 1u : i > 0, go);
+                tc_commit(&sh.o_step[t][b], go);
+                if (last) tc_commit(&sh.ring.empty[v_stage], go);
+                p_phase ^= 1u << b;
+            }
+            if (i + 2 < steps) {
+                if (first) tile(k_stage);
+                const uint32_t k0 = k_desc + k_stage * (kStage >> 4) + half * kHalf, to = s_columns + b * kTcStep;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                    tc_mma_ss(to, q0 + at, k0 + at, kScores, k > 0, go);
+                }
+                tc_commit(&sh.s_full[t][b], go);
+                if (last) tc_commit(&sh.ring.empty[k_stage], go);
             }
         }
-        tc_commit(&sh.o_full[T], go);
+        tc_commit(&sh.o_full[t], go);
     }
     template <typename Walk>
     __device__ __forceinline__ void run(const PagedArgs &a, Walk &walk) {
@@ -278,14 +270,11 @@ struct TcIssuer {
         int kt0, kt1, out;
         while (tc_uniform(walk.next(a, it, kt0, kt1, out))) {
             wait(&sh.q_full, stays++);
-            if (tc_uniform(it.r1 - it.r0 > 128))
-                stay<true>(it, kt0, tc_uniform(kt1 - kt0));
-            else
-                stay<false>(it, kt0, tc_uniform(kt1 - kt0));
+            stay(it, kt0, tc_uniform(kt1 - kt0), tc_uniform(it.r1 - it.r0 > 128));
         }
         // every product issued completes before TMEM is freed
-        tc_commit(&sh.drain[T], tc_elect());
-        mbar_wait_bounded(&sh.drain[T], 0, kTilePolls);
+        tc_commit(&sh.drain[t], tc_elect());
+        mbar_wait_bounded(&sh.drain[t], 0, kTilePolls);
     }
 };
 
@@ -335,10 +324,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // registers: 384 x 168 at launch = 128 x 104 + 256 x 200
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (any && warp == 8)
-            TcIssuer<D, BF16, 0>(sh, smem_u32(sq), ring).run(a, walk);
-        else if (any && warp == 9)
-            TcIssuer<D, BF16, 1>(sh, smem_u32(sq), ring).run(a, walk);
+        if (any && warp < 10)
+            TcIssuer<D, BF16>(sh, smem_u32(sq), ring, warp - 8).run(a, walk);
         else if (any)
             load_tiles<D, kStages, 2>(a, walk, sh.ring, ring, &k_map, &v_map, heads_outer, 128, warp - 10);
     } else {
@@ -347,6 +334,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int t = warp >> 2, wrow = (warp & 3) * 32, lrow = wrow + lane;
         const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16), o_at = s_at + kO;
         const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
+        // 16-byte piece c of row r of 128 rows as the MMAs read them
+        auto row_piece = [](uint8_t *rows, int r, int c) {
+            return reinterpret_cast<uint4 *>(rows + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        };
+        constexpr int kLanes = D / 8, kPass = 32 / kLanes;  // lanes to a row of D 16-bit values, rows of a warp's access
         const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
         uint32_t steps[2] = {0, 0}, stays = 0;  // steps: through each S buffer
         PagedItem it;
@@ -361,23 +353,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool warp_live = row - lane < it.r1;
             int lo, hi;
             paged_row_range(a, it, row, lo, hi);
-            // Q rows into shared memory; with the same rows in both streams each loads half the columns
+            // Q rows into shared memory, whole rows by neighbouring lanes: a warp's own 32, or 16
+            // of those that both streams have
             if (!both) asm volatile("bar.sync 1, 256;" ::: "memory");  // both streams have left the last stay
+            uint8_t *rows_at = sq + (both ? t * 128 * D * 2 : 0);
             {
-                const uint16_t *q = static_cast<const uint16_t *>(a.q) +
-                                    (live ? paged_row_offset(a, it, row, a.q_row, a.q_head) : 0);
-                uint8_t *dst = sq + (both ? t * 128 * D * 2 : 0);
-                const int c0 = both ? 0 : t * (D / 16);
-                uint4 w[D / 8];
+                const int first = (both ? wrow : warp * 16) + lane / kLanes, c = lane % kLanes;
+                const int row0 = it.r0 + (both ? t * 128 : 0);
+                const int end = both ? 32 : 16;
+#pragma unroll 1
+                for (int i0 = 0; i0 < end; i0 += 4 * kPass) {
+                    uint4 w[4];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    w[i] = live && (both || i < D / 16) ? __ldg(reinterpret_cast<const uint4 *>(q + (c0 + i) * 8))
-                                                        : make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = row0 + first + i0 + i * kPass;
+                        w[i] = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < it.r1)
+                            w[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) +
+                                                                         paged_row_offset(a, it, r, a.q_row, a.q_head)) + c);
+                    }
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const int c = c0 + i;
-                    if (both || i < D / 16)
-                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + lrow * 128 + (((c & 7) ^ (lrow & 7)) << 4)) =
+                    for (int i = 0; i < 4; ++i)
+                        *row_piece(rows_at, first + i0 + i * kPass, c) =
                             make_uint4(w[i].x ^ flip, w[i].y ^ flip, w[i].z ^ flip, w[i].w ^ flip);
                 }
             }
@@ -485,45 +482,73 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if ((both || t == 0) && warp_live) {
                 const float inv = out >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
                 float probe = 0.0f;
-                float *po = a.parts[1].o + (static_cast<int64_t>(max(out, 0)) * kTcItem + row - it.r0) * D;
+                const int64_t part_row = static_cast<int64_t>(max(out, 0)) * kTcItem + row - it.r0;
                 const int64_t at = live ? paged_row_offset(a, it, row, a.out_row, D) : 0;
+                // a row's 16 columns from TMEM go to memory from here when the rows are few; else by way
+                // of the warp's Q rows (done with), so that neighbouring lanes store whole rows: all
+                // 16-bit columns at once, partials in two halves
+                const int passes = out >= 0 ? 2 : 1, each = D / 16 / passes;
+                for (int pass = 0; pass < passes; ++pass) {
 #pragma unroll 1
-                for (int i = 0; i < D / 16; ++i) {
-                    float o[16];
-                    tc_ld16(o_at + 16 * i, o);
-                    tc_ld_wait();
-                    if (!both) {
+                    for (int i = pass * each; i < (pass + 1) * each; ++i) {
+                        float o[16];
+                        tc_ld16(o_at + 16 * i, o);
+                        tc_ld_wait();
+                        if (!both) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float4 x = swap[(i * 4 + k) * 128 + lrow];
-                            o[4 * k] = o[4 * k] * mine_w + x.x * other_w;
-                            o[4 * k + 1] = o[4 * k + 1] * mine_w + x.y * other_w;
-                            o[4 * k + 2] = o[4 * k + 2] * mine_w + x.z * other_w;
-                            o[4 * k + 3] = o[4 * k + 3] * mine_w + x.w * other_w;
+                            for (int k = 0; k < 4; ++k) {
+                                const float4 x = swap[(i * 4 + k) * 128 + lrow];
+                                o[4 * k] = o[4 * k] * mine_w + x.x * other_w;
+                                o[4 * k + 1] = o[4 * k + 1] * mine_w + x.y * other_w;
+                                o[4 * k + 2] = o[4 * k + 2] * mine_w + x.z * other_w;
+                                o[4 * k + 3] = o[4 * k + 3] * mine_w + x.w * other_w;
+                            }
                         }
-                    }
-                    if (out >= 0) {
-                        if (live)
+                        if (out >= 0) {
 #pragma unroll
-                            for (int k = 0; k < 16; k += 4)
-                                *reinterpret_cast<float4 *>(po + 16 * i + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                    } else {
-                        uint32_t w[8];
+                            for (int k = 0; k < 4; ++k) {
+                                const float4 x = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                                if (both)
+                                    *reinterpret_cast<float4 *>(row_piece(rows_at, lrow, (i - pass * each) * 4 + k)) = x;
+                                else if (live)
+                                    *reinterpret_cast<float4 *>(a.parts[1].o + part_row * D + 16 * i + 4 * k) = x;
+                            }
+                        } else {
+                            uint32_t w[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float x = o[2 * k] * inv, y = o[2 * k + 1] * inv;
-                            probe += 0.0f * x + 0.0f * y;
-                            w[k] = tc_pack<BF16>(x, y);
+                            for (int k = 0; k < 8; ++k) {
+                                const float x = o[2 * k] * inv, y = o[2 * k + 1] * inv;
+                                probe += 0.0f * x + 0.0f * y;
+                                w[k] = tc_pack<BF16>(x, y);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const uint4 x = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                                if (both)
+                                    *row_piece(rows_at, lrow, 2 * i + k) = x;
+                                else if (live)
+                                    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at + 16 * i + 8 * k) = x;
+                            }
                         }
-                        if (live)
-#pragma unroll
-                            for (int k = 0; k < 8; k += 4)
-                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at + 16 * i + 2 * k) =
-                                    make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (both) {
+#pragma unroll 2
+                        for (int i = 0; i < 32; i += kPass) {
+                            const int lr = wrow + i + lane / kLanes, c = lane % kLanes, r = it.r0 + t * 128 + lr;
+                            if (r >= it.r1) continue;
+                            const uint4 x = *row_piece(rows_at, lr, c);
+                            if (out >= 0)
+                                reinterpret_cast<uint4 *>(a.parts[1].o + (static_cast<int64_t>(out) * kTcItem + r - it.r0) * D +
+                                                          pass * (D / 2))[c] = x;
+                            else
+                                reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) +
+                                                          paged_row_offset(a, it, r, a.out_row, D))[c] = x;
+                        }
+                        __syncwarp();
+                    }
                 }
-                if (out >= 0 && live) *reinterpret_cast<float2 *>(a.parts[1].ml + (po - a.parts[1].o) / D * 2) = make_float2(m, l);
+                if (out >= 0 && live) *reinterpret_cast<float2 *>(a.parts[1].ml + part_row * 2) = make_float2(m, l);
                 // rows with a value that is not finite are done again, key by key
                 unsigned odd = __ballot_sync(0xffffffffu, live && out < 0 && !(probe == 0.0f));
                 while (odd) {
