@@ -388,8 +388,9 @@ __device__ __forceinline__ void paged_zero_rows(const PagedArgs &a) {
 // stages that the other warps release.
 
 constexpr int kTileKeys = 128;
-constexpr int kRowsItem = 64;  // rows of an item: mma.sync kernel
-constexpr int kTcItem = 256;   // tcgen05 kernel
+constexpr int kRowsItem = 32;  // rows of an item: mma.sync kernel, the most of a request there
+// of the tcgen05 kernel: two streams of 128 rows, or of fp32 rows one
+__host__ __device__ constexpr int tc_item(int mode) { return mode == PAGED_F32 ? 128 : 256; }
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTilePolls = 1u << 21;
 

@@ -1,6 +1,6 @@
-// Attention over the paged cache for few rows per (request, kv head): single tokens,
-// draft blocks, and fp32 rows of any count.  The mathematics and the work split are
-// those at the head of paged_attention.cu, with 64 rows to an item.
+// Attention over the paged cache for few rows per (request, kv head), as of single
+// tokens.  The mathematics and the work split are
+// those at the head of paged_attention.cu, with 32 rows to an item.
 //
 // One CTA per SM: four warps load key and value tiles by TMA into a ring of six
 // stages (about 190 KB in flight, which is what covers HBM's latency), eight warps
@@ -8,8 +8,7 @@
 // tile; each has the running maximum, sum and O of its rows over its keys, so the
 // warps meet only at the end of a stay.  S = Q K^T and O += P V are m16n8k16 MMAs.
 // At one token and four heads to a kv head the MMAs, softmax and loads of a warp
-// hide under the 2800 cycles that a tile takes to come from HBM; fp32 rows do
-// twice the MMAs and are bound by them from 64 rows on.
+// hide under the 2800 cycles that a tile takes to come from HBM.
 #include "paged_attention.cuh"
 
 namespace bd {
@@ -127,8 +126,7 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
     rows_load_q<D, MODE>(a, it, area, sh);
     rows_meet();
     const bool live = it.r0 + rw * 16 < it.r1;
-    // Q fragments stay in registers where there is room for them beside S and O
-    constexpr bool kHold = !F32 && KK <= 32;
+    constexpr bool kHold = !F32;  // Q fragments stay in registers where there is room for them beside S and O
     uint32_t q[kHold ? D / 16 : 1][4];
     const int q_at = rw * 16 + (mi & 1) * 8 + r8;
     if (kHold)
@@ -409,10 +407,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             if (tid == 0 && part >= 0 && (part & 1)) a.parts[0].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
             if (rows <= 16)
                 rows_stay<D, MODE, 1>(a, it, kt0, kt1, part, sh, stages, area, place);
-            else if (rows <= 32)
-                rows_stay<D, MODE, 2>(a, it, kt0, kt1, part, sh, stages, area, place);
             else
-                rows_stay<D, MODE, 4>(a, it, kt0, kt1, part, sh, stages, area, place);
+                rows_stay<D, MODE, 2>(a, it, kt0, kt1, part, sh, stages, area, place);
             place += 2 * (kt1 - kt0);
         }
         if (sh.ring.abort && tid == 0) set_flag(a.flags, BD_FLAG_TIMEOUT);
