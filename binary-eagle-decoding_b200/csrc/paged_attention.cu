@@ -13,10 +13,10 @@
 // the cache's type (relative 2^-11 and 2^-8 at most, the size of the output's own
 // rounding); the row sum adds the fp32 values.
 //
-// Two kernels: requests of up to kSplitRows rows per kv head run on mma.sync
-// (paged_attention_rows.cu), the others on tcgen05 (paged_attention_tc.cu).  A batch
-// may hold both kinds; lengths are read on the device, so no launch parameter depends
-// on them.
+// Two kernels: requests of up to 32 (or 64) rows per kv head, and fp32 rows of any count,
+// run on mma.sync (paged_attention_rows.cu), the others on tcgen05
+// (paged_attention_tc.cu).  A batch may hold both kinds; lengths are read on the device,
+// so no launch parameter depends on them.
 //
 // Work split, in each: a unit is one 128-key tile of one item, an item is up to M
 // rows of one (request, kv head).  The units of all items, in the order (request,
@@ -32,10 +32,13 @@
 
 namespace bd {
 
-// 32 requests over 4096 keys each, 128 columns, rows per kv head: 16: 101 us on mma.sync
-// and 110 on tcgen05, 32: 119 and 111, 64: 165 and 115; one request, 16 and 64 rows:
-// 17.4 and 22.1, 21.5 and 23.3; 64 columns, 32 rows: 92 and 96.
-constexpr int kSplitRows = kRowsItem;
+// Which kernel, for fp16 and bf16 rows: mma.sync up to 32 rows per kv head (32 fp16
+// requests over 4096 keys each, 128 columns, 16 rows: 101 us there and 110 on tcgen05,
+// 32 rows: 119 and 111, 64: 165 and 115; 64 columns, 32 rows: 92 and 96).  With so few
+// (request, kv head) pairs a CTA has one stay, whose latency counts, and mma.sync keeps
+// up to 64 rows (16 tokens of 4 heads over 4096 keys, 1 request: 21.5 and 23.3 us, 2:
+// 26.6 and 23.8).
+constexpr int kFewPairs = 8;
 
 // Joins the partials of the items that lie across CTAs: CTA (x, y) those of the item
 // that CTA x (of the first kernel, then of the second) left open, a warp to a row, 8
@@ -54,7 +57,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
     if (a.zero_fill && blockIdx.y == 0) paged_zero_rows<D, MODE>(a);
     if (open.last < 0) return;
     const PagedItem &it = open.it;
-    const int rows = set ? tc_item(MODE) : kRowsItem;
+    const int rows = set ? kTcItem : a.item_rows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int V = D / 32;  // values of a lane
     for (int row = it.r0 + blockIdx.y * (kJoinThreads / 32) + warp; row < it.r1; row += kJoinBlocks * (kJoinThreads / 32)) {
@@ -187,7 +190,7 @@ static size_t carve(PagedArgs &a, void *workspace, int head_dim) {
     };
     const size_t ctas = device_sms();
     for (int set = 0; set < 2; ++set) {
-        const size_t rows = 2 * ctas * (set ? tc_item(PAGED_F16) : kRowsItem);
+        const size_t rows = 2 * ctas * (set ? kTcItem : rows_item(true));
         a.parts[set].o = static_cast<float *>(take(rows * head_dim * sizeof(float)));
         a.parts[set].ml = static_cast<float *>(take(rows * 2 * sizeof(float)));
         a.parts[set].open = static_cast<PagedOpen *>(take(ctas * sizeof(PagedOpen)));
@@ -255,13 +258,15 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     a.out_row = static_cast<int64_t>(p->heads) * p->head_dim;
     a.zero_fill = p->zero_fill;
     a.flags = p->flags;
+    const bool wide = mode == PAGED_F32 || static_cast<int64_t>(a.requests) * a.kv_heads <= kFewPairs;
+    a.item_rows = rows_item(wide);
+    a.split_rows = mode == PAGED_F32 ? INT_MAX : a.item_rows;
     // a batch that cannot hold a longer request needs the one kernel
-    const bool tiles = std::min<int64_t>(a.longest, p->rows) * a.groups > kSplitRows;
-    a.split_rows = kSplitRows;
+    const bool tiles = std::min<int64_t>(a.longest, p->rows) * a.groups > a.split_rows;
     PagedMaps maps;
     if (!paged_maps(a, p->head_dim, mode == PAGED_BF16, maps)) return BD_ERR_ALIGNMENT;
     const int ctas = device_sms();
-    int st = launch_paged_rows(a, maps, p->head_dim, mode, ctas, stream);
+    int st = launch_paged_rows(a, maps, p->head_dim, mode, wide, ctas, stream);
     if (!st && tiles) st = launch_paged_tc(a, maps, p->head_dim, mode, ctas, stream);
     if (st) return st;
     return p->head_dim == 64 ? launch_join<64>(a, mode, tiles ? 2 : 1, ctas, stream)

@@ -34,6 +34,7 @@ struct PagedArgs {
     void *out;
     int64_t out_row;  // heads stand head_dim apart
     int zero_fill;
+    int item_rows;   // rows of an item of the mma.sync kernel
     int split_rows;  // requests of more rows per kv head go to the tcgen05 kernel (INT_MAX: none)
     // partials of the two kernels: [2 x CTAs][rows of an item][head_dim] and [..][2], and what to join
     struct Parts {
@@ -388,9 +389,9 @@ __device__ __forceinline__ void paged_zero_rows(const PagedArgs &a) {
 // stages that the other warps release.
 
 constexpr int kTileKeys = 128;
-constexpr int kRowsItem = 32;  // rows of an item: mma.sync kernel, the most of a request there
-// of the tcgen05 kernel: two streams of 128 rows, or of fp32 rows one
-__host__ __device__ constexpr int tc_item(int mode) { return mode == PAGED_F32 ? 128 : 256; }
+// rows of an item: mma.sync kernel (`wide`: also takes requests of up to 64 rows)
+__host__ __device__ constexpr int rows_item(bool wide) { return wide ? 64 : 32; }
+constexpr int kTcItem = 256;  // tcgen05 kernel: two streams of 128
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTilePolls = 1u << 21;
 
@@ -493,7 +494,8 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
 
 // Tensor maps of the caches; false when their strides cannot be expressed.
 bool paged_maps(const PagedArgs &a, int head_dim, bool bf16, PagedMaps &maps);
-int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream);
+int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, bool wide, int ctas,
+                      cudaStream_t stream);
 int launch_paged_tc(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream);
 
 }  // namespace bd

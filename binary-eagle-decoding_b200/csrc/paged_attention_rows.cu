@@ -1,6 +1,6 @@
 // Attention over the paged cache for few rows per (request, kv head), as of single
-// tokens.  The mathematics and the work split are
-// those at the head of paged_attention.cu, with 32 rows to an item.
+// tokens, and for fp32 rows of any count.  The mathematics and the work split are
+// those at the head of paged_attention.cu, with 32 or 64 rows to an item.
 //
 // One CTA per SM: four warps load key and value tiles by TMA into a ring of six
 // stages (about 190 KB in flight, which is what covers HBM's latency), eight warps
@@ -8,12 +8,14 @@
 // tile; each has the running maximum, sum and O of its rows over its keys, so the
 // warps meet only at the end of a stay.  S = Q K^T and O += P V are m16n8k16 MMAs.
 // At one token and four heads to a kv head the MMAs, softmax and loads of a warp
-// hide under the 2800 cycles that a tile takes to come from HBM.
+// hide under the 2800 cycles that a tile takes to come from HBM; fp32 rows do twice the
+// MMAs and are bound by them from 64 rows on (24 blocks: 51 % of the MMA pipe).
 #include "paged_attention.cuh"
 
 namespace bd {
 
 constexpr int kRowsWarps = 8;
+constexpr int kPlane = 64;  // rows of a plane of Q in shared memory
 constexpr int kRowsExtra = 1;  // a stay's Q, joining and output, in units
 constexpr int kRowsThreads = 384;
 
@@ -32,11 +34,11 @@ constexpr size_t rows_smem() {
     return 1024 + static_cast<size_t>(rows_stages<D>()) * tile_bytes<D>() + rows_area<D>();
 }
 static_assert(rows_smem<128>() + sizeof(TileRing) + 1024 <= 232448, "one CTA's shared memory");
-static_assert(rows_area<128>() >= 2 * kRowsItem * 128 * 2 && rows_area<64>() >= 2 * kRowsItem * 64 * 2, "Q fits");
+static_assert(rows_area<128>() >= 2 * kPlane * 128 * 2 && rows_area<64>() >= 2 * kPlane * 64 * 2, "Q fits");
 
 struct RowsShared {
     TileRing ring;
-    float fold[kRowsItem];
+    float fold[kPlane];
     PagedShared walk;
 };
 
@@ -99,16 +101,16 @@ __device__ __forceinline__ void rows_load_q(const PagedArgs &a, const PagedItem 
             split_half2(u.z * down, u.w * down, hi.y, lo.y);
             split_half2(v.x * down, v.y * down, hi.z, lo.z);
             split_half2(v.z * down, v.w * down, hi.w, lo.w);
-            const uint32_t to = tile_piece<kRowsItem>(r, part * kChunks + i);
+            const uint32_t to = tile_piece<kPlane>(r, part * kChunks + i);
             *reinterpret_cast<uint4 *>(area + to) = hi;
-            *reinterpret_cast<uint4 *>(area + kRowsItem * D * 2 + to) = lo;
+            *reinterpret_cast<uint4 *>(area + kPlane * D * 2 + to) = lo;
         }
     } else {
         const uint16_t *q = static_cast<const uint16_t *>(a.q) + at;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const uint4 w = live ? __ldg(reinterpret_cast<const uint4 *>(q) + i) : make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4 *>(area + tile_piece<kRowsItem>(r, part * kChunks + i)) = w;
+            *reinterpret_cast<uint4 *>(area + tile_piece<kPlane>(r, part * kChunks + i)) = w;
         }
     }
 }
@@ -126,12 +128,13 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
     rows_load_q<D, MODE>(a, it, area, sh);
     rows_meet();
     const bool live = it.r0 + rw * 16 < it.r1;
-    constexpr bool kHold = !F32;  // Q fragments stay in registers where there is room for them beside S and O
+    // Q fragments stay in registers where there is room for them beside S and O
+    constexpr bool kHold = !F32 && KK <= 32;
     uint32_t q[kHold ? D / 16 : 1][4];
     const int q_at = rw * 16 + (mi & 1) * 8 + r8;
     if (kHold)
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) ldmatrix_x4(q[kHold ? d : 0], area + tile_piece<kRowsItem>(q_at, 2 * d + (mi >> 1)));
+        for (int d = 0; d < D / 16; ++d) ldmatrix_x4(q[kHold ? d : 0], area + tile_piece<kPlane>(q_at, 2 * d + (mi >> 1)));
     float fold[2];
     int lo[2], hi[2];
 #pragma unroll
@@ -171,11 +174,11 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
                         x1[i] = q[kHold ? 2 * d + 1 : 0][i];
                     }
                 } else {
-                    ldmatrix_x4(x0, area + tile_piece<kRowsItem>(q_at, 4 * d + (mi >> 1)));
-                    ldmatrix_x4(x1, area + tile_piece<kRowsItem>(q_at, 4 * d + 2 + (mi >> 1)));
+                    ldmatrix_x4(x0, area + tile_piece<kPlane>(q_at, 4 * d + (mi >> 1)));
+                    ldmatrix_x4(x1, area + tile_piece<kPlane>(q_at, 4 * d + 2 + (mi >> 1)));
                     if (F32) {
-                        ldmatrix_x4(y0, area + kRowsItem * D * 2 + tile_piece<kRowsItem>(q_at, 4 * d + (mi >> 1)));
-                        ldmatrix_x4(y1, area + kRowsItem * D * 2 + tile_piece<kRowsItem>(q_at, 4 * d + 2 + (mi >> 1)));
+                        ldmatrix_x4(y0, area + kPlane * D * 2 + tile_piece<kPlane>(q_at, 4 * d + (mi >> 1)));
+                        ldmatrix_x4(y1, area + kPlane * D * 2 + tile_piece<kPlane>(q_at, 4 * d + 2 + (mi >> 1)));
                     }
                 }
 #pragma unroll
@@ -330,7 +333,7 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
             const int row = it.r0 + rw * 16 + g + 8 * r;
             if (row >= it.r1) continue;
             if (part >= 0) {
-                const int64_t at = static_cast<int64_t>(part) * kRowsItem + row - it.r0;
+                const int64_t at = static_cast<int64_t>(part) * a.item_rows + row - it.r0;
                 float *po = a.parts[0].o + at * D;
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
@@ -369,7 +372,8 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
     rows_meet();  // the area is free for the next Q
 }
 
-template <int D, int MODE>
+// WIDE: items of 64 rows.  A kernel of its own: its larger code costs the others 8 %.
+template <int D, int MODE, bool WIDE>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     paged_rows_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       int heads_outer) {
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     __syncthreads();
     grid_wait();
     grid_launch_dependents();
-    PagedWalk<kRowsItem, kTileKeys, kRowsExtra, false> walk;
+    PagedWalk<rows_item(WIDE), kTileKeys, kRowsExtra, false> walk;
     if (tid == 0) a.parts[0].open[blockIdx.x].last = -1;
     if (!walk.begin(a, sh.walk, blockIdx.x, gridDim.x)) return;
     // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
@@ -407,31 +411,40 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             if (tid == 0 && part >= 0 && (part & 1)) a.parts[0].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
             if (rows <= 16)
                 rows_stay<D, MODE, 1>(a, it, kt0, kt1, part, sh, stages, area, place);
-            else
+            else if (!WIDE || rows <= 32)
                 rows_stay<D, MODE, 2>(a, it, kt0, kt1, part, sh, stages, area, place);
+            else
+                rows_stay<D, MODE, WIDE ? 4 : 2>(a, it, kt0, kt1, part, sh, stages, area, place);
             place += 2 * (kt1 - kt0);
         }
         if (sh.ring.abort && tid == 0) set_flag(a.flags, BD_FLAG_TIMEOUT);
     }
 }
 
-template <int D, int MODE>
+template <int D, int MODE, bool WIDE>
 static int launch_rows(const PagedArgs &a, const PagedMaps &maps, int ctas, cudaStream_t stream) {
-    if (cudaFuncSetAttribute(paged_rows_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(rows_smem<D>())) != cudaSuccess)
+    auto kernel = paged_rows_kernel<D, MODE, WIDE>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rows_smem<D>())) != cudaSuccess)
         return BD_ERR_LAUNCH;
-    return launch_pdl(paged_rows_kernel<D, MODE>, dim3(ctas), dim3(kRowsThreads), rows_smem<D>(), stream, a, maps.k, maps.v,
-                      maps.heads_outer);
+    return launch_pdl(kernel, dim3(ctas), dim3(kRowsThreads), rows_smem<D>(), stream, a, maps.k, maps.v, maps.heads_outer);
 }
 
-int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream) {
+template <int D, int MODE>
+static int launch_rows(const PagedArgs &a, const PagedMaps &maps, bool wide, int ctas, cudaStream_t stream) {
+    if constexpr (MODE != PAGED_F32)  // whose items are always wide
+        if (!wide) return launch_rows<D, MODE, false>(a, maps, ctas, stream);
+    return launch_rows<D, MODE, true>(a, maps, ctas, stream);
+}
+
+int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, bool wide, int ctas,
+                      cudaStream_t stream) {
     if (head_dim == 64)
-        return mode == PAGED_F32   ? launch_rows<64, PAGED_F32>(a, maps, ctas, stream)
-               : mode == PAGED_F16 ? launch_rows<64, PAGED_F16>(a, maps, ctas, stream)
-                                   : launch_rows<64, PAGED_BF16>(a, maps, ctas, stream);
-    return mode == PAGED_F32   ? launch_rows<128, PAGED_F32>(a, maps, ctas, stream)
-           : mode == PAGED_F16 ? launch_rows<128, PAGED_F16>(a, maps, ctas, stream)
-                               : launch_rows<128, PAGED_BF16>(a, maps, ctas, stream);
+        return mode == PAGED_F32   ? launch_rows<64, PAGED_F32>(a, maps, wide, ctas, stream)
+               : mode == PAGED_F16 ? launch_rows<64, PAGED_F16>(a, maps, wide, ctas, stream)
+                                   : launch_rows<64, PAGED_BF16>(a, maps, wide, ctas, stream);
+    return mode == PAGED_F32   ? launch_rows<128, PAGED_F32>(a, maps, wide, ctas, stream)
+           : mode == PAGED_F16 ? launch_rows<128, PAGED_F16>(a, maps, wide, ctas, stream)
+                               : launch_rows<128, PAGED_BF16>(a, maps, wide, ctas, stream);
 }
 
 }  // namespace bd

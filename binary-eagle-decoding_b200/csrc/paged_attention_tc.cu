@@ -1,6 +1,8 @@
-// Attention over the paged cache on the 5th-generation tensor cores (tcgen05, TMEM).
-// The mathematics, the item / unit / range split and the joining of partials are those
-// of paged_attention.cu, with 256 rows to an item (fp32 rows: 128).
+// Attention over the paged cache on the 5th-generation tensor cores (tcgen05, TMEM), for
+// fp16 and bf16 rows.  The mathematics, the item / unit / range split and the joining
+// of partials are those of paged_attention.cu, with 256 rows to an item.  (fp32 rows,
+// as hi and lo halves of Q and P, ran here 14 % faster at 24 blocks of 64 rows, but the
+// accumulators in TMEM truncate: 3.9e-6 off after 2000 keys against 1e-6 there.)
 //
 // One CTA per SM.  Two streams of work alternate on the tensor pipe:
 //   * an item of more than 128 rows: stream t has rows [128 t, 128 t + 128), and both
@@ -46,7 +48,7 @@ struct TcShared {
     // o_step is for the products of a step, o_full for those of a stay.
     uint64_t q_full, s_full[2][2], p_full[2][2], o_step[2][2], o_full[2], drain[2];
     uint32_t tmem;
-    float2 ml[128];  // at the end of a stay (at its begin the fold of fp32 rows)
+    float2 ml[128];
     PagedShared walk;
 };
 
@@ -185,7 +187,7 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
 template <int D, int MODE>
 struct TcIssuer {
     static constexpr int kStages = tc_stages<D>(), kStage = tile_bytes<D>();
-    static constexpr bool BF16 = MODE == PAGED_BF16, F32 = MODE == PAGED_F32;
+    static constexpr bool BF16 = MODE == PAGED_BF16;
     static constexpr uint32_t kScores = tc_idesc(BF16, kTcStep, false), kValues = tc_idesc(BF16, D, true);
     static constexpr uint32_t kHalf = kTcStep * 128 >> 4;  // of a tile, in descriptor units
     TcShared &sh;
@@ -245,10 +247,6 @@ struct TcIssuer {
 #pragma unroll
                 for (int k = 0; k < kTcStep / 16; ++k)
                     tc_mma_ts(o_columns, from + k * 8, v0 + k * (2048 >> 4), kValues, k > 0 ? 1u : i > 0, go);
-                if (F32)  // the low halves of P
-#pragma unroll
-                    for (int k = 0; k < kTcStep / 16; ++k)
-                        tc_mma_ts(o_columns, from + 32 + k * 8, v0 + k * (2048 >> 4), kValues, 1u, go);
                 tc_commit(&sh.o_step[t][b], go);
                 if (last) tc_commit(&sh.ring.empty[v_stage], go);
                 p_phase ^= 1u << b;
@@ -261,12 +259,6 @@ struct TcIssuer {
                     const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
                     tc_mma_ss(to, q0 + at, k0 + at, kScores, k > 0, go);
                 }
-                if (F32)  // the low halves of Q
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t at = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                        tc_mma_ss(to, q0 + (128 * D * 2 >> 4) + at, k0 + at, kScores, 1u, go);
-                    }
                 tc_commit(&sh.s_full[t][b], go);
                 if (last) tc_commit(&sh.ring.empty[k_stage], go);
             }
@@ -288,41 +280,10 @@ struct TcIssuer {
     }
 };
 
-// Two planes of fp32 Q rows, fp16 hi + lo of the row over a power of two (so that the
-// halves of values up to 1 lose nothing to fp16's range), 16 rows to a warp; fold = scale
-// x log2 e x that power.
-template <int D>
-__device__ __forceinline__ void tc_load_f32(const PagedArgs &a, const PagedItem &it, int warp, uint8_t *sq, float *fold) {
-    constexpr int kLanes = D / 4, kPass = 32 / kLanes;  // lanes to a row, rows of a warp's access
-    const int lane = threadIdx.x & 31, c = lane % kLanes;
-#pragma unroll 2
-    for (int i = 0; i < 16; i += kPass) {
-        const int lr = warp * 16 + i + lane / kLanes, r = it.r0 + lr;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r < it.r1)
-            x = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) +
-                                                       paged_row_offset(a, it, r, a.q_row, a.q_head)) + c);
-        float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-#pragma unroll
-        for (int d = kLanes / 2; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-        int e = 0;
-        if (big > 0.0f && big < INFINITY) e = min(max(ilogbf(big) + 1, -100), 126);
-        const float down = copysignf(ldexpf(1.0f, -e), a.scale_log2);  // the scale's sign goes into Q
-        uint2 hi, lo;
-        split_half2(x.x * down, x.y * down, hi.x, lo.x);
-        split_half2(x.z * down, x.w * down, hi.y, lo.y);
-        uint8_t *to = sq + (c >> 4) * 16384 + lr * 128 + ((((c >> 1) & 7) ^ (lr & 7)) << 4) + (c & 1) * 8;
-        *reinterpret_cast<uint2 *>(to) = hi;
-        *reinterpret_cast<uint2 *>(to + 128 * D * 2) = lo;
-        if (c == 0) fold[lr] = fmaxf(fabsf(a.scale_log2) * ldexpf(1.0f, e), 1e-37f);
-    }
-}
-
 template <int D, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_tc_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                     int heads_outer) {
-    constexpr bool F32 = MODE == PAGED_F32;
     constexpr int kStages = tc_stages<D>();
     constexpr uint32_t kO = 256;  // TMEM columns: two S buffers of each stream (P over them), O at 256 and 384
     extern __shared__ uint8_t tc_raw[];
@@ -358,7 +319,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = sh.tmem;
     grid_wait();
     grid_launch_dependents();
-    PagedWalk<tc_item(MODE), kTileKeys, kTcExtra, true> walk;
+    PagedWalk<kTcItem, kTileKeys, kTcExtra, true> walk;
     if (tid == 0) a.parts[1].open[blockIdx.x].last = -1;
     const bool any = walk.begin(a, sh.walk, blockIdx.x, gridDim.x);
     // registers: 384 x 168 at launch = 128 x 104 + 256 x 200
@@ -373,7 +334,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // -------------------------------------------------- softmax: a thread to a row
         const int t = warp >> 2, wrow = (warp & 3) * 32, lrow = wrow + lane;
         const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16), o_at = s_at + kO;
-        float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
+        const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
         // 16-byte piece c of row r of 128 rows as the MMAs read them
         auto row_piece = [](uint8_t *rows, int r, int c) {
             return reinterpret_cast<uint4 *>(rows + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -397,9 +358,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // of those that both streams have
             if (!both) asm volatile("bar.sync 1, 256;" ::: "memory");  // both streams have left the last stay
             uint8_t *rows_at = sq + (both ? t * 128 * D * 2 : 0);
-            if (F32) {
-                tc_load_f32<D>(a, it, warp, sq, &sh.ml[0].x);
-            } else {
+            {
                 const int first = (both ? wrow : warp * 16) + lane / kLanes, c = lane % kLanes;
                 const int row0 = it.r0 + (both ? t * 128 : 0);
                 const int end = both ? 32 : 16;
@@ -425,10 +384,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             if (lane == 0) tile_arrive(&sh.q_full);
 
-            if (F32) {
-                asm volatile("bar.sync 1, 256;" ::: "memory");  // fold is written
-                c = (&sh.ml[0].x)[lrow];
-            }
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < count; ++i) {
                 const int buffer = i & 1;
@@ -479,20 +434,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const float base = m == -INFINITY ? 0.0f : m;
                     const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
                     float2 sum[4];
-                    uint32_t w[32], low[F32 ? 32 : 1];
+                    uint32_t w[32];
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
                         const float *x = &s[k >> 4][2 * (k & 15)];
                         float2 p = __ffma2_rn(make_float2(x[0], x[1]), c2, base2);
                         p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
                         sum[k & 3] = k < 4 ? p : __fadd2_rn(sum[k & 3], p);
-                        if (F32)
-                            split_half2(p.x, p.y, w[k], low[F32 ? k : 0]);
-                        else
-                            w[k] = tc_pack<MODE>(p.x, p.y);
+                        w[k] = tc_pack<MODE>(p.x, p.y);
                     }
                     tc_st32(at, w);
-                    if constexpr (F32) tc_st32(at + 32, low);
                     const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
                     l += all.x + all.y;
                     tc_st_wait();
@@ -532,7 +483,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if ((both || t == 0) && warp_live) {
                 const float inv = out >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
                 float probe = 0.0f;
-                const int64_t part_row = static_cast<int64_t>(max(out, 0)) * tc_item(MODE) + row - it.r0;
+                const int64_t part_row = static_cast<int64_t>(max(out, 0)) * kTcItem + row - it.r0;
                 const int64_t at = live ? paged_row_offset(a, it, row, a.out_row, D) : 0;
                 // a row's 16 columns from TMEM go to memory from here when the rows are few; else by way
                 // of the warp's Q rows (done with), so that neighbouring lanes store whole rows: all
@@ -563,13 +514,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 else if (live)
                                     *reinterpret_cast<float4 *>(a.parts[1].o + part_row * D + 16 * i + 4 * k) = x;
                             }
-                        } else if (F32) {
-#pragma unroll
-                            for (int k = 0; k < 16; k += 4) {
-                                const float4 x = make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv);
-                                probe += 0.0f * x.x + 0.0f * x.y + 0.0f * x.z + 0.0f * x.w;
-                                if (live) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at + 16 * i + k) = x;
-                            }
                         } else {
                             uint32_t w[8];
 #pragma unroll
@@ -596,7 +540,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             if (r >= it.r1) continue;
                             const uint4 x = *row_piece(rows_at, lr, c);
                             if (out >= 0)
-                                reinterpret_cast<uint4 *>(a.parts[1].o + (static_cast<int64_t>(out) * tc_item(MODE) + r - it.r0) * D +
+                                reinterpret_cast<uint4 *>(a.parts[1].o + (static_cast<int64_t>(out) * kTcItem + r - it.r0) * D +
                                                           pass * (D / 2))[c] = x;
                             else
                                 reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) +
@@ -641,12 +585,10 @@ static int launch_tc(const PagedArgs &a, const PagedMaps &maps, int ctas, cudaSt
 
 int launch_paged_tc(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream) {
     if (head_dim == 64)
-        return mode == PAGED_F32   ? launch_tc<64, PAGED_F32>(a, maps, ctas, stream)
-               : mode == PAGED_F16 ? launch_tc<64, PAGED_F16>(a, maps, ctas, stream)
-                                   : launch_tc<64, PAGED_BF16>(a, maps, ctas, stream);
-    return mode == PAGED_F32   ? launch_tc<128, PAGED_F32>(a, maps, ctas, stream)
-           : mode == PAGED_F16 ? launch_tc<128, PAGED_F16>(a, maps, ctas, stream)
-                               : launch_tc<128, PAGED_BF16>(a, maps, ctas, stream);
+        return mode == PAGED_F16 ? launch_tc<64, PAGED_F16>(a, maps, ctas, stream)
+                                 : launch_tc<64, PAGED_BF16>(a, maps, ctas, stream);
+    return mode == PAGED_F16 ? launch_tc<128, PAGED_F16>(a, maps, ctas, stream)
+                             : launch_tc<128, PAGED_BF16>(a, maps, ctas, stream);
 }
 
 }  // namespace bd

@@ -696,7 +696,6 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
 
 
 _PLAN_ROWS = 4096  # rows that the plan's one CTA fills itself
-_SPLIT_ROWS = 32  # rows per kv head above which a request goes to the tcgen05 kernel
 
 
 def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor, flags: Flags | None = None) -> None:
@@ -795,7 +794,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
         min(longest, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
         flags.ptr))
-    both = min(longest, rows) * (heads // kv_heads) > _SPLIT_ROWS
+    both = dtype is not torch.float32 and min(longest, rows) * (heads // kv_heads) > (64 if requests * kv_heads <= 8 else 32)
     _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device), kernels=2 + both)
     if own:
         flags.check()
