@@ -392,8 +392,11 @@ extern "C" int bd_page_plan(const int32_t *context, const int32_t *count, int re
     a.rows = rows;
     a.rows_here = rows <= kPlanRows;
     a.flags = flags;
-    // barriers and scans are shorter with fewer warps
-    const int threads = requests <= 256 && rows <= 1024 ? 256 : kPlanThreads;
+    // Barriers and scans are shorter with fewer warps, rows want a thread each: 32 requests
+    // with 512 rows take 6.6 us with 256 threads, 5.9 us with 512.
+    const int threads = requests <= 256 && rows <= 256   ? 256
+                        : requests <= 512 && rows <= 1024 ? 512
+                                                          : kPlanThreads;
     int st = launch_pdl(page_plan_kernel, dim3(1), dim3(threads), 0, stream, a);
     if (st || a.rows_here) return st;
     // twice the stretches of an average request, so that longer ones spread too
