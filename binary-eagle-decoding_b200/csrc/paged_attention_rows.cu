@@ -116,8 +116,10 @@ __device__ __forceinline__ void rows_load_q(const PagedArgs &a, const PagedItem 
 }
 
 // One stay on an item by the computing warps.  place0: the ring place of its first tile.
+// Returns which of the item's rows (of the warp's 16, by bits) hold a value that is not
+// finite.
 template <int D, int MODE, int RW>
-__device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &it, int kt0, int kt1, int part, RowsShared &sh,
+__device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedItem &it, int kt0, int kt1, int part, RowsShared &sh,
                                           uint8_t *stages, uint8_t *area, uint32_t place0) {
     constexpr int KW = kRowsWarps / RW, KK = kTileKeys / KW;  // key parts, keys of a warp
     constexpr int kStages = rows_stages<D>();
@@ -326,8 +328,9 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
                 for (int i = 0; i < 4; ++i) o[n][i] = o[n][i] * mine[i >> 1] + w[(n * 4 + i) * 32] * other[i >> 1];
         }
     }
+    unsigned odd_rows = 0;
     if (kw == 0 && live) {
-        bool odd[2] = {false, false};  // a value that is not finite
+        bool odd[2] = {false, false};
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int row = it.r0 + rw * 16 + g + 8 * r;
@@ -355,21 +358,14 @@ __device__ __forceinline__ void rows_stay(const PagedArgs &a, const PagedItem &i
             }
             odd[r] = !(probe == 0.0f);
         }
-        // rows with a value that is not finite are done again, key by key
-        __syncwarp();
-        unsigned rows[2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) rows[r] = __ballot_sync(0xffffffffu, odd[r]);
-        while (rows[0] | rows[1]) {
-            const int r = rows[0] ? 0 : 1, gg = (__ffs(rows[0] ? rows[0] : rows[1]) - 1) >> 2;
-            if (r == 0)
-                rows[0] &= ~(0xFu << (4 * gg));
-            else
-                rows[1] &= ~(0xFu << (4 * gg));
-            paged_slow_row<D, MODE>(a, it, it.r0 + rw * 16 + gg + 8 * r);
+        for (int r = 0; r < 2; ++r) {
+            const unsigned vote = __ballot_sync(0xffffffffu, odd[r]);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) odd_rows |= (vote >> (4 * x) & 0xF) ? 1u << (x + 8 * r) : 0u;
         }
     }
-    rows_meet();  // the area is free for the next Q
+    return odd_rows;
 }
 
 // WIDE: items of 64 rows.  A kernel of its own: its larger code costs the others 8 %.
@@ -397,24 +393,34 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     PagedWalk<rows_item(WIDE), kTileKeys, kRowsExtra, false> walk;
     if (tid == 0) a.parts[0].open[blockIdx.x].last = -1;
     if (!walk.begin(a, sh.walk, blockIdx.x, gridDim.x)) return;
-    // registers: 384 x 168 at launch = 128 x 72 + 256 x 216
+    // registers: 384 x 168 at launch = 128 x 56 + 256 x 224
     if (warp >= kRowsWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         load_tiles<D, kStages, 4>(a, walk, sh.ring, stages, &k_map, &v_map, heads_outer, -1, warp - kRowsWarps);
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         uint32_t place = 0;
         PagedItem it;
         int kt0, kt1, part;
         while (walk.next(a, it, kt0, kt1, part)) {
             const int rows = it.r1 - it.r0;
             if (tid == 0 && part >= 0 && (part & 1)) a.parts[0].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
-            if (rows <= 16)
-                rows_stay<D, MODE, 1>(a, it, kt0, kt1, part, sh, stages, area, place);
-            else if (!WIDE || rows <= 32)
-                rows_stay<D, MODE, 2>(a, it, kt0, kt1, part, sh, stages, area, place);
-            else
-                rows_stay<D, MODE, WIDE ? 4 : 2>(a, it, kt0, kt1, part, sh, stages, area, place);
+            unsigned odd;
+            int row0;  // of the warp
+            if (rows <= 16) {
+                odd = rows_stay<D, MODE, 1>(a, it, kt0, kt1, part, sh, stages, area, place);
+                row0 = 0;
+            } else if (!WIDE || rows <= 32) {
+                odd = rows_stay<D, MODE, 2>(a, it, kt0, kt1, part, sh, stages, area, place);
+                row0 = warp % 2 * 16;
+            } else {
+                odd = rows_stay<D, MODE, WIDE ? 4 : 2>(a, it, kt0, kt1, part, sh, stages, area, place);
+                row0 = warp % 4 * 16;
+            }
+            // rows with a value that is not finite are done again, key by key
+            __syncwarp();
+            for (; odd; odd &= odd - 1) paged_slow_row<D, MODE>(a, it, it.r0 + row0 + __ffs(odd) - 1);
+            rows_meet();  // the area is free for the next Q
             place += 2 * (kt1 - kt0);
         }
         if (sh.ring.abort && tid == 0) set_flag(a.flags, BD_FLAG_TIMEOUT);
