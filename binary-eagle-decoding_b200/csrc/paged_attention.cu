@@ -39,6 +39,11 @@ namespace bd {
 // up to 64 rows (16 tokens of 4 heads over 4096 keys, 1 request: 21.5 and 23.3 us, 2:
 // 26.6 and 23.8).
 constexpr int kFewPairs = 8;
+// A batch that may hold longer requests pays 4 to 8 us for the mma.sync kernel's launch
+// even if it has no rows there.  With up to 256 pairs all go to tcgen05 (two chunks of 1024
+// tokens and 6 single tokens over 4096 keys, 8 kv heads: 149 us instead of 181, 14: 181 and
+// 202, 30: 251 and 246, 62: 386 and 326; 32 x 17 tokens over 2048 keys: 76 and 84).
+constexpr int kOneKernelPairs = 256;
 
 // Joins the partials of the items that lie across CTAs: CTA (x, y) those of the item
 // that CTA x (of the first kernel, then of the second) left open, a warp to a row, 8
@@ -51,7 +56,7 @@ template <int D, int MODE>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int ctas) {
     grid_wait();
     grid_launch_dependents();
-    const int set = blockIdx.x >= ctas, cta = blockIdx.x - set * ctas;
+    const int set = a.split_rows == 0 || blockIdx.x >= ctas, cta = blockIdx.x % ctas;
     const PagedArgs::Parts &parts = a.parts[set];
     const PagedOpen open = parts.open[cta];
     if (a.zero_fill && blockIdx.y == 0) paged_zero_rows<D, MODE>(a);
@@ -258,17 +263,20 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     a.out_row = static_cast<int64_t>(p->heads) * p->head_dim;
     a.zero_fill = p->zero_fill;
     a.flags = p->flags;
-    const bool wide = mode == PAGED_F32 || static_cast<int64_t>(a.requests) * a.kv_heads <= kFewPairs;
+    const int64_t pairs = static_cast<int64_t>(a.requests) * a.kv_heads;
+    const bool wide = mode == PAGED_F32 || pairs <= kFewPairs;
     a.item_rows = rows_item(wide);
     a.split_rows = mode == PAGED_F32 ? INT_MAX : a.item_rows;
     // a batch that cannot hold a longer request needs the one kernel
     const bool tiles = std::min<int64_t>(a.longest, p->rows) * a.groups > a.split_rows;
+    const bool few = !tiles || pairs > kOneKernelPairs;
+    if (!few) a.split_rows = 0;  // the tcgen05 kernel has them all
     PagedMaps maps;
     if (!paged_maps(a, p->head_dim, mode == PAGED_BF16, maps)) return BD_ERR_ALIGNMENT;
     const int ctas = device_sms();
-    int st = launch_paged_rows(a, maps, p->head_dim, mode, wide, ctas, stream);
+    int st = few ? launch_paged_rows(a, maps, p->head_dim, mode, wide, ctas, stream) : BD_OK;
     if (!st && tiles) st = launch_paged_tc(a, maps, p->head_dim, mode, ctas, stream);
     if (st) return st;
-    return p->head_dim == 64 ? launch_join<64>(a, mode, tiles ? 2 : 1, ctas, stream)
-                             : launch_join<128>(a, mode, tiles ? 2 : 1, ctas, stream);
+    return p->head_dim == 64 ? launch_join<64>(a, mode, few + tiles, ctas, stream)
+                             : launch_join<128>(a, mode, few + tiles, ctas, stream);
 }

@@ -35,7 +35,7 @@ struct PagedArgs {
     int64_t out_row;  // heads stand head_dim apart
     int zero_fill;
     int item_rows;   // rows of an item of the mma.sync kernel
-    int split_rows;  // requests of more rows per kv head go to the tcgen05 kernel (INT_MAX: none)
+    int split_rows;  // requests of more rows per kv head go to the tcgen05 kernel (INT_MAX: none, 0: all)
     // partials of the two kernels: [2 x CTAs][rows of an item][head_dim] and [..][2], and what to join
     struct Parts {
         float *o, *ml;

@@ -363,10 +363,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int row0 = it.r0 + (both ? t * 128 : 0);
                 const int end = both ? 32 : 16;
 #pragma unroll 1
-                for (int i0 = 0; i0 < end; i0 += 4 * kPass) {
-                    uint4 w[4];
+                for (int i0 = 0; i0 < end; i0 += 8 * kPass) {
+                    uint4 w[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 8; ++i) {
                         const int r = row0 + first + i0 + i * kPass;
                         w[i] = make_uint4(0u, 0u, 0u, 0u);
                         if (r < it.r1)
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                                          paged_row_offset(a, it, r, a.q_row, a.q_head)) + c);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 8; ++i)
                         *row_piece(rows_at, first + i0 + i * kPass, c) =
                             make_uint4(w[i].x ^ flip, w[i].y ^ flip, w[i].z ^ flip, w[i].w ^ flip);
                 }
