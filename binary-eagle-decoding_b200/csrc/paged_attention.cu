@@ -67,8 +67,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
     constexpr int V = D / 32;  // values of a lane
     for (int row = it.r0 + blockIdx.y * (kJoinThreads / 32) + warp; row < it.r1; row += kJoinBlocks * (kJoinThreads / 32)) {
         auto place = [&](int p) { return static_cast<int64_t>(2 * p + (p == cta)) * rows + row - it.r0; };
-        float m = -INFINITY;
-        for (int p = cta + lane; p <= open.last; p += 32) m = fmaxf(m, parts.ml[place(p) * 2]);
+        auto stats = [&](int p) {
+            return p <= open.last ? *reinterpret_cast<const float2 *>(parts.ml + place(p) * 2) : make_float2(-INFINITY, 0.0f);
+        };
+        float2 ml = stats(cta + lane);
+        float m = ml.x;
+        for (int p = cta + 32 + lane; p <= open.last; p += 32) m = fmaxf(m, stats(p).x);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         const float base = m == -INFINITY ? 0.0f : m;
@@ -76,28 +80,28 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = 0.0f;
         for (int p0 = cta; p0 <= open.last; p0 += 32) {
-            float w = 0.0f, lw = 0.0f;
-            if (p0 + lane <= open.last) {
-                const float2 ml = *reinterpret_cast<const float2 *>(parts.ml + place(p0 + lane) * 2);
-                w = exp2_fast(ml.x - base);
-                lw = w * ml.y;
-            }
+            if (p0 != cta) ml = stats(p0 + lane);
+            const float w = exp2_fast(ml.x - base), lw = w * ml.y;
             const int n = min(32, open.last - p0 + 1);
-#pragma unroll 8
-            for (int j = 0; j < n; ++j) {
-                const float wj = __shfl_sync(0xffffffffu, w, j);
-                l += __shfl_sync(0xffffffffu, lw, j);
-                const float *po = parts.o + place(p0 + j) * D + lane * V;
-                if (V == 4) {
-                    const float4 x = *reinterpret_cast<const float4 *>(po);
-                    o[0] += wj * x.x;
-                    o[1] += wj * x.y;
-                    o[V - 2] += wj * x.z;
-                    o[V - 1] += wj * x.w;
-                } else {
-                    const float2 x = *reinterpret_cast<const float2 *>(po);
-                    o[0] += wj * x.x;
-                    o[1] += wj * x.y;
+            // O of eight partials in flight
+            for (int j0 = 0; j0 < n; j0 += 8) {
+                float x[8][V];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (j0 + j >= n) break;
+                    const float *po = parts.o + place(p0 + j0 + j) * D + lane * V;
+                    if (V == 4)
+                        *reinterpret_cast<float4 *>(x[j]) = *reinterpret_cast<const float4 *>(po);
+                    else
+                        *reinterpret_cast<float2 *>(x[j]) = *reinterpret_cast<const float2 *>(po);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (j0 + j >= n) break;
+                    const float wj = __shfl_sync(0xffffffffu, w, j0 + j);
+                    l += __shfl_sync(0xffffffffu, lw, j0 + j);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] += wj * x[j][i];
                 }
             }
         }

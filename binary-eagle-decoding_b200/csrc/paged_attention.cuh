@@ -165,8 +165,8 @@ struct PagedWalk {
     }
 
     // Cost of one kv head of request b, a request to a lane; those of many items by the whole warp.
-    static __device__ __forceinline__ int64_t request_cost(const PagedArgs &a, int b) {
-        PagedRequest r{};
+    static __device__ __forceinline__ int64_t request_cost(const PagedArgs &a, int b, PagedRequest &r) {
+        r = PagedRequest{};
         if (b < a.requests) {
             r = paged_request(a, b);
             if (r.bad) set_flag(a.flags, BD_FLAG_BAD_LENGTH);
@@ -216,43 +216,76 @@ struct PagedWalk {
         tiles = request_tiles(a, r);
     }
 
-    // Places the walk at the begin of this CTA's range of `ctas` equal ones; false when it is empty.
+    // Dividing 64-bit values takes some 300 cycles at a CTA's begin.
+    static __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+        return (x | y) >> 32 ? x / y : static_cast<int64_t>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
+    }
+
+    // This CTA's range [u, u + len) of `ctas` equal ones of `total`; false when it is empty.
+    __device__ __forceinline__ bool range(int64_t total, int ctas, int64_t &u) {
+        per = static_cast<int>(divide(total + ctas - 1, ctas));
+        u = static_cast<int64_t>(cta) * per;
+        len = static_cast<int>(min(static_cast<int64_t>(per), total - u));
+        return u < total;
+    }
+
+    // Places the walk at the begin of this CTA's range; false when it is empty.
     __device__ __forceinline__ bool begin(const PagedArgs &a, PagedShared &sh, int cta_, int ctas) {
         cta = cta_;
         const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31;
-        int64_t each = request_cost(a, tid), total, sum;
-        int64_t incl = scan(each * a.kv_heads, sh, total);
-        for (int b0 = n; b0 < a.requests; b0 += n) {
-            scan(request_cost(a, b0 + tid) * a.kv_heads, sh, sum);
-            total += sum;
-        }
-        per = static_cast<int>((total + ctas - 1) / ctas);
-        const int64_t u = static_cast<int64_t>(cta) * per;
-        if (u >= total) return false;
-        len = static_cast<int>(min(static_cast<int64_t>(per), total - u));
-        // the request around u
-        int64_t before = 0;
-        sum = total;
-        for (int b0 = 0; b0 < a.requests; b0 += n) {
-            if (a.requests > n) {
-                each = request_cost(a, b0 + tid);
-                incl = scan(each * a.kv_heads, sh, sum);
+        int64_t total, u, each, rest;  // each: cost of one kv head of the request around u
+        if (a.requests <= 32) {  // every warp for itself, without a barrier
+            PagedRequest mine;
+            const int64_t cost = request_cost(a, lane, mine);
+            int64_t incl = cost * a.kv_heads;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += o;
             }
-            if (before + incl - each * a.kv_heads <= u && u < before + incl) {
-                sh.b = b0 + tid;
-                sh.before = before + incl - each * a.kv_heads;
-                sh.each = each;
+            total = __shfl_sync(0xffffffffu, incl, 31);
+            if (!range(total, ctas, u)) return false;
+            b = __ffs(__ballot_sync(0xffffffffu, u < incl)) - 1;
+            each = __shfl_sync(0xffffffffu, cost, b);
+            rest = u - (__shfl_sync(0xffffffffu, incl, b) - each * a.kv_heads);
+            r.row0 = __shfl_sync(0xffffffffu, mine.row0, b);
+            r.count = __shfl_sync(0xffffffffu, mine.count, b);
+            r.context = __shfl_sync(0xffffffffu, mine.context, b);
+            r.bad = false;  // it has rows
+            tiles = request_tiles(a, r);
+        } else {
+            PagedRequest unused;
+            int64_t sum, cost = request_cost(a, tid, unused);
+            int64_t incl = scan(cost * a.kv_heads, sh, total);
+            for (int b0 = n; b0 < a.requests; b0 += n) {
+                scan(request_cost(a, b0 + tid, unused) * a.kv_heads, sh, sum);
+                total += sum;
             }
-            before += sum;
-            if (u < before) break;
+            if (!range(total, ctas, u)) return false;
+            int64_t before = 0;
+            sum = total;
+            for (int b0 = 0; b0 < a.requests; b0 += n) {
+                if (a.requests > n) {
+                    cost = request_cost(a, b0 + tid, unused);
+                    incl = scan(cost * a.kv_heads, sh, sum);
+                }
+                if (before + incl - cost * a.kv_heads <= u && u < before + incl) {
+                    sh.b = b0 + tid;
+                    sh.before = before + incl - cost * a.kv_heads;
+                    sh.each = cost;
+                }
+                before += sum;
+                if (u < before) break;
+            }
+            __syncthreads();
+            b = sh.b;
+            each = sh.each;
+            rest = u - sh.before;
+            set_request(a);
         }
-        __syncthreads();
-        b = sh.b;
-        int64_t rest = u - sh.before;
-        set_request(a);
         // its kv head, and the item: 32 at a time, every warp for itself
-        h = static_cast<int>(rest / sh.each);
-        rest -= h * sh.each;
+        h = static_cast<int>(divide(rest, each));
+        rest -= h * each;
         for (int i0 = 0;; i0 += 32) {
             const int mine = i0 + lane < tiles ? cost(a, r, i0 + lane) : 0;
             int end = mine;
