@@ -794,7 +794,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
         min(longest, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
         flags.ptr))
-    both = dtype is not torch.float32 and min(longest, rows) * (heads // kv_heads) > (64 if requests * kv_heads <= 8 else 32)
+    pairs = requests * kv_heads  # up to 256 of them have one kernel beside the join, whatever their lengths
+    both = dtype is not torch.float32 and pairs > 256 and min(longest, rows) * (heads // kv_heads) > 32
     _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device), kernels=2 + both)
     if own:
         flags.check()

@@ -481,6 +481,73 @@ def test_attention_repeats_bit_for_bit(ops):
             assert torch.equal(batch.run(ops), first)
 
 
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("requests, heads, kv_heads, head_dim, counts", [
+    (32, 16, 8, 64, (1, 40, 3)), (33, 16, 8, 64, (1, 40, 3)), (40, 24, 8, 128, (0, 1, 17, 100)), (400, 2, 1, 64, (1, 0, 70)),
+    (900, 2, 1, 64, (1, 1, 33, 2))])
+def test_attention_of_many_requests(ops, row_type, requests, heads, kv_heads, head_dim, counts):
+    """Short and long requests side by side, on either side of 32 requests, 256 (request,
+    kv head) pairs and a block's threads, where the split of the work takes another way."""
+    lengths = [((37 * b) % 211, counts[b % len(counts)]) for b in range(requests)]
+    check(ops, Batch(lengths, heads, kv_heads, head_dim, 16, row_type, seed=19))
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("order", [(0, 1, 2), (0, 2, 1), (1, 0, 2), (1, 2, 0), (2, 0, 1), (2, 1, 0)])
+@pytest.mark.parametrize("count", [3, 40])
+def test_caches_in_any_order_of_their_axes(ops, row_type, order, count):
+    """Pages, slots and heads lie in any order, keys and values in one buffer: the store
+    and the attention see the same cache."""
+    batch = Batch([(150, count), (9, count)], 6, 2, 64, 16, row_type, seed=20)
+    want = batch.run(ops)
+    shape = [batch.k.shape[i] for i in order]
+    both = torch.zeros((*shape[:2], 2, shape[2], 64), dtype=batch.k.dtype, device=DEV)
+    back = [order.index(i) for i in range(3)] + [3]
+    k, v = (both[:, :, i].permute(back) for i in range(2))
+    rows = batch.k.flatten(0, 1), batch.v.flatten(0, 1)
+    ops.paged_store(*rows, torch.arange(rows[0].shape[0], dtype=torch.int32, device=DEV), k, v)
+    assert torch.equal(k, batch.k) and torch.equal(v, batch.v)
+    batch.k, batch.v = k, v
+    assert torch.equal(batch.run(ops), want)
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+def test_longest_bounds_the_requests(ops, row_type):
+    """A bound that holds changes no value; a request beyond it is left out, with a flag."""
+    lib = submodule("_lib")
+    batch = Batch([(70, 5), (300, 90), (20, 1)], 8, 2, 64, 32, row_type, seed=21)
+    want, bound = batch.expected()
+    for longest in (90, 91, 2 ** 31 - 1, 2 ** 40):
+        assert bool(((batch.run(ops, longest=longest).double() - want).abs() <= bound).all())
+    for longest in (1, 5, 89):
+        flags = ops.Flags(DEV)
+        got = batch.run(ops, longest=longest, flags=flags)
+        assert int(flags.tensor.item()) == lib.FLAG_BAD_LENGTH
+        row = 0
+        for _, count in batch.lengths:
+            here = slice(row, row + count)
+            if count <= longest:
+                assert bool(((got[here].double() - want[here]).abs() <= bound[here]).all())
+            else:
+                assert not got[here].any()
+            row += count
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+def test_many_calls_in_a_row_end_alike(ops, row_type):
+    """Calls of every kernel queued one behind the other: none runs out of its waits."""
+    batches = [Batch([(500, 1000), (0, 900)], 16, 4, 128, 64, row_type, seed=22),
+               Batch([(900, 17)] * 9, 16, 4, 64, 16, row_type, seed=23), Batch([(4000, 1)] * 40, 16, 8, 64, 16, row_type, seed=24)]
+    flags = ops.Flags(DEV)
+    first = [batch.run(ops, flags=flags) for batch in batches]
+    for i in range(60):
+        for batch, want in zip(batches, first):
+            got = batch.run(ops, flags=flags)
+            if i % 20 == 19:
+                assert torch.equal(got, want)
+    flags.check()
+
+
 def test_calls_on_streams_and_in_graphs_do_not_meet(ops):
     """Two captured graphs replayed at once on their own streams, with lengths changed
     between replays, beside eager calls of the same operators."""
