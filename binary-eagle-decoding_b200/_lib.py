@@ -208,7 +208,7 @@ SIGNATURES = {
     "bd_paged_store": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, P, c_int64, c_int, c_int, c_int,
                                c_int64, P, P, P, P, c_int, P, P]),
     "bd_paged_attention_workspace_bytes": (c_size_t, [c_int]),
-    "bd_paged_attention": (c_int, [ctypes.POINTER(PagedAttentionArgs), P]),
+    "bd_paged_attention": (c_int, [P, P]),  # PagedAttentionArgs, or its bytes
     "bd_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "bd_attention_decode": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, P,
                                     P, c_size_t, P]),

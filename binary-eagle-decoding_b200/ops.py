@@ -607,15 +607,23 @@ class PagePlan(NamedTuple):
     slots: Tensor
 
 
+_I32 = torch.int32
+_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _raw_stream(index: int) -> int:
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def _int32(name: str, t: Tensor, shape: tuple[int, ...]) -> None:
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}")
 
 
 def _table_ld(table: Tensor, requests: int) -> int:
     """The row stride of a table of pages."""
     shape = table.shape
-    if table.dtype is torch.int32 and len(shape) == 2 and shape[0] == requests and shape[1] > 0:
+    if table.dtype is _I32 and len(shape) == 2 and shape[0] == requests and shape[1] > 0:
         row, column = table.stride()
         if (column == 1 or shape[1] == 1) and (row >= shape[1] or requests < 2):
             return max(row, shape[1])
@@ -631,10 +639,10 @@ def _cache_shape(k_cache: Tensor, v_cache: Tensor) -> torch.Size:
     return shape
 
 
-def _one_device(device: torch.device, *others: Tensor) -> None:
-    if device.type != "cuda":
+def _one_device(index: int, *others: Tensor) -> None:
+    """The tensors are on the CUDA device of this index (what ``get_device`` gives)."""
+    if index < 0:
         raise ValueError("bitdraft kernels take CUDA tensors")
-    index = device.index
     for t in others:
         if t.get_device() != index:
             raise ValueError("all tensors must be on one device")
@@ -678,18 +686,18 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
         raise ValueError("page_size must be a power of two from 8 to 256")
     if rows < 0:
         raise ValueError("rows must not be negative")
-    device = context.device
-    _one_device(device, count, table, owned, free, top, owned_out, top_out)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = context.get_device()
+    _one_device(index, count, table, owned, free, top, owned_out, top_out)
+    if index != _DEVICE():
+        with torch.cuda.device(index):
             return page_plan(context, count, table, owned, free, top, page_size, rows, pool_pages, owned_out, top_out, flags)
     starts, positions, slots = context.new_empty(requests + 1), context.new_empty(rows), context.new_empty(rows)
     own = flags is None
-    flags = flags or Flags(device)
+    flags = flags or Flags(context.device)
     _lib.call("bd_page_plan", context.data_ptr(), count.data_ptr(), requests, page_size, pool_pages, table.data_ptr(), ld,
               table.shape[1], owned.data_ptr(), owned_out.data_ptr(), free.data_ptr(), capacity, top.data_ptr(),
-              top_out.data_ptr(), starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), rows, flags.ptr,
-              _stream(device), kernels=1 if rows <= _PLAN_ROWS else 2)
+              top_out.data_ptr(), starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), rows,
+              flags.tensor.data_ptr(), _raw_stream(index), kernels=1 if rows <= _PLAN_ROWS else 2)
     if own:
         flags.check()
     return PagePlan(starts, positions, slots)
@@ -717,16 +725,16 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
         raise ValueError("k and v need unit stride within a head")
     rows = shape[0]
     _int32("slots", slots, (rows,))
-    device = k.device
-    _one_device(device, v, slots, k_cache, v_cache)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = k.get_device()
+    _one_device(index, v, slots, k_cache, v_cache)
+    if index != _DEVICE():
+        with torch.cuda.device(index):
             return paged_store(k, v, slots, k_cache, v_cache, flags)
     own = flags is None
-    flags = flags or Flags(device)
+    flags = flags or Flags(k.device)
     _lib.call("bd_paged_store", k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, _ROW_TYPE[dtype],
               slots.data_ptr(), rows, kv_heads, head_dim, page_size, pages, k_cache.data_ptr(), _Strides(*k_strides),
-              v_cache.data_ptr(), _Strides(*v_strides), _CACHE_TYPE[k_cache.dtype], flags.ptr, _stream(device))
+              v_cache.data_ptr(), _Strides(*v_strides), _CACHE_TYPE[k_cache.dtype], flags.tensor.data_ptr(), _raw_stream(index))
     if own:
         flags.check()
 
@@ -772,31 +780,31 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         longest = rows
     elif longest < 1:
         raise ValueError("longest must be at least 1")
-    device = q.device
-    _one_device(device, k_cache, v_cache, table, context, starts)
+    index = q.get_device()
+    _one_device(index, k_cache, v_cache, table, context, starts)
     fresh = out is None
-    if not fresh and (out.shape != shape or out.dtype is not dtype or out.device != device or not out.is_contiguous()):
+    if not fresh and (out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous()):
         raise ValueError("out must be contiguous and like q")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    if index != _DEVICE():
+        with torch.cuda.device(index):
             return paged_attention(q, k_cache, v_cache, table, context, starts, causal, window or None, scale, longest or 1,
                                    out, flags)
     if fresh:
         out = q.new_empty(shape)
     nbytes = _lib.size("bd_paged_attention_workspace_bytes", head_dim)
     # a buffer of this call: concurrent streams and captured graphs share none
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = context.new_empty(nbytes // 4)
     own = flags is None
-    flags = flags or Flags(device)
-    args = _lib.PagedAttentionArgs.from_buffer_copy(_lib.PAGED_ATTENTION_ARGS.pack(
+    flags = flags or Flags(q.device)
+    args = _lib.PAGED_ATTENTION_ARGS.pack(
         q.data_ptr(), q_row, q_head, _ROW_TYPE[dtype], k_cache.data_ptr(), v_cache.data_ptr(), *k_strides[:3],
         *v_strides[:3], _CACHE_TYPE[k_cache.dtype], page_size, pages, table.data_ptr(), ld, table.shape[1],
         context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
         min(longest, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
-        flags.ptr))
+        flags.tensor.data_ptr())
     pairs = requests * kv_heads  # up to 256 of them have one kernel beside the join, whatever their lengths
     both = dtype is not torch.float32 and pairs > 256 and min(longest, rows) * (heads // kv_heads) > 32
-    _lib.call("bd_paged_attention", _lib.ctypes.byref(args), _stream(device), kernels=2 + both)
+    _lib.call("bd_paged_attention", args, _raw_stream(index), kernels=2 + both)
     if own:
         flags.check()
     return out
