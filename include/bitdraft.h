@@ -468,8 +468,12 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * A request whose lengths do not fit (rows, table_width, longest) is left out
  * (BD_FLAG_BAD_LENGTH); keys on a page outside the pool count as zeros
  * (BD_FLAG_BAD_PAGE); entries of pages that no token sees are not read.  What the
- * cache holds at keys that a row does not see never reaches it, not even as NaN.
- * The workspace needs no clearing; calls that overlap on the GPU need their own. */
+ * cache holds at keys that a row does not see never reaches it, not even as NaN:
+ * a row with a value that is not finite is done again over its own keys, by one warp
+ * and so slowly (about 0.1 us a key).  Strides as at bd_paged_store; caches are read
+ * by TMA, so strides that a tensor map cannot hold are BD_ERR_ALIGNMENT too.
+ * The workspace needs no clearing; calls that overlap on the GPU need their own.
+ * Results do not depend on what else the GPU runs: partials are joined in order. */
 #define BD_F16 0
 #define BD_BF16 1
 #define BD_F32 2
