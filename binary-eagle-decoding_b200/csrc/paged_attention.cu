@@ -13,8 +13,8 @@
 // the cache's type (relative 2^-11 and 2^-8 at most, the size of the output's own
 // rounding); the row sum adds the fp32 values.
 //
-// Two kernels: requests of up to 32 (or 64) rows per kv head, and fp32 rows of any count,
-// run on mma.sync (paged_attention_rows.cu), the others on tcgen05
+// Two kernels: requests of up to 16 rows per kv head (32 with 64 columns), and fp32 rows of
+// any count, run on mma.sync (paged_attention_rows.cu), the others on tcgen05
 // (paged_attention_tc.cu).  A batch may hold both kinds; lengths are read on the device,
 // so no launch parameter depends on them.
 //
@@ -32,13 +32,6 @@
 
 namespace bd {
 
-// Which kernel, for fp16 and bf16 rows: mma.sync up to 32 rows per kv head (32 fp16
-// requests over 4096 keys each, 128 columns, 16 rows: 101 us there and 110 on tcgen05,
-// 32 rows: 119 and 111, 64: 165 and 115; 64 columns, 32 rows: 92 and 96).  With so few
-// (request, kv head) pairs a CTA has one stay, whose latency counts, and mma.sync keeps
-// up to 64 rows (16 tokens of 4 heads over 4096 keys, 1 request: 21.5 and 23.3 us, 2:
-// 26.6 and 23.8).
-constexpr int kFewPairs = 8;
 // A batch that may hold longer requests pays 4 to 8 us for the mma.sync kernel's launch
 // even if it has no rows there.  With up to 256 pairs all go to tcgen05 (two chunks of 1024
 // tokens and 6 single tokens over 4096 keys, 8 kv heads: 149 us instead of 181, 14: 181 and
@@ -199,7 +192,7 @@ static size_t carve(PagedArgs &a, void *workspace, int head_dim) {
     };
     const size_t ctas = device_sms();
     for (int set = 0; set < 2; ++set) {
-        const size_t rows = 2 * ctas * (set ? kTcItem : rows_item(true));
+        const size_t rows = 2 * ctas * (set ? kTcItem : kRowsItemMax);
         a.parts[set].o = static_cast<float *>(take(rows * head_dim * sizeof(float)));
         a.parts[set].ml = static_cast<float *>(take(rows * 2 * sizeof(float)));
         a.parts[set].open = static_cast<PagedOpen *>(take(ctas * sizeof(PagedOpen)));
@@ -268,8 +261,7 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     a.zero_fill = p->zero_fill;
     a.flags = p->flags;
     const int64_t pairs = static_cast<int64_t>(a.requests) * a.kv_heads;
-    const bool wide = mode == PAGED_F32 || pairs <= kFewPairs;
-    a.item_rows = rows_item(wide);
+    a.item_rows = rows_item(p->head_dim, mode);
     a.split_rows = mode == PAGED_F32 ? INT_MAX : a.item_rows;
     // a batch that cannot hold a longer request needs the one kernel
     const bool tiles = std::min<int64_t>(a.longest, p->rows) * a.groups > a.split_rows;
@@ -278,7 +270,7 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     PagedMaps maps;
     if (!paged_maps(a, p->head_dim, mode == PAGED_BF16, maps)) return BD_ERR_ALIGNMENT;
     const int ctas = device_sms();
-    int st = few ? launch_paged_rows(a, maps, p->head_dim, mode, wide, ctas, stream) : BD_OK;
+    int st = few ? launch_paged_rows(a, maps, p->head_dim, mode, ctas, stream) : BD_OK;
     if (!st && tiles) st = launch_paged_tc(a, maps, p->head_dim, mode, ctas, stream);
     if (st) return st;
     return p->head_dim == 64 ? launch_join<64>(a, mode, few + tiles, ctas, stream)

@@ -422,8 +422,14 @@ __device__ __forceinline__ void paged_zero_rows(const PagedArgs &a) {
 // stages that the other warps release.
 
 constexpr int kTileKeys = 128;
-// rows of an item: mma.sync kernel (`wide`: also takes requests of up to 64 rows)
-__host__ __device__ constexpr int rows_item(bool wide) { return wide ? 64 : 32; }
+// Rows of an item in the mma.sync kernel.  For fp16 and bf16 rows also the most that a
+// request has there per kv head; more go to tcgen05 (32 fp16 requests over 4096 keys each,
+// 128 columns: 16 rows take 99 us on mma.sync and 101 on tcgen05, 32 rows 115 and 102; 64
+// requests over 2048 keys, 64 columns: 32 rows 88 and 100).
+constexpr int kRowsItemMax = 64;
+__host__ __device__ constexpr int rows_item(int head_dim, int mode) {
+    return mode == PAGED_F32 ? kRowsItemMax : (head_dim == 64 ? 32 : 16);
+}
 constexpr int kTcItem = 256;  // tcgen05 kernel: two streams of 128
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTilePolls = 1u << 21;
@@ -527,8 +533,7 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
 
 // Tensor maps of the caches; false when their strides cannot be expressed.
 bool paged_maps(const PagedArgs &a, int head_dim, bool bf16, PagedMaps &maps);
-int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, bool wide, int ctas,
-                      cudaStream_t stream);
+int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream);
 int launch_paged_tc(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream);
 
 }  // namespace bd

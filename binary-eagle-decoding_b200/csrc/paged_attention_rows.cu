@@ -1,6 +1,6 @@
 // Attention over the paged cache for few rows per (request, kv head), as of single
 // tokens, and for fp32 rows of any count.  The mathematics and the work split are
-// those at the head of paged_attention.cu, with 32 or 64 rows to an item.
+// those at the head of paged_attention.cu, with 16, 32 or 64 rows to an item.
 //
 // One CTA per SM: four warps load key and value tiles by TMA into a ring of six
 // stages (about 190 KB in flight, which is what covers HBM's latency), eight warps
@@ -368,8 +368,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
     return odd_rows;
 }
 
-// WIDE: items of 64 rows.  A kernel of its own: its larger code costs the others 8 %.
-template <int D, int MODE, bool WIDE>
+template <int D, int MODE>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     paged_rows_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       int heads_outer) {
@@ -390,7 +389,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     __syncthreads();
     grid_wait();
     grid_launch_dependents();
-    PagedWalk<rows_item(WIDE), kTileKeys, kRowsExtra, false> walk;
+    constexpr int M = rows_item(D, MODE);
+    PagedWalk<M, kTileKeys, kRowsExtra, false> walk;
     if (tid == 0) a.parts[0].open[blockIdx.x].last = -1;
     if (!walk.begin(a, sh.walk, blockIdx.x, gridDim.x)) return;
     // registers: 384 x 168 at launch = 128 x 56 + 256 x 224
@@ -407,14 +407,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             if (tid == 0 && part >= 0 && (part & 1)) a.parts[0].open[blockIdx.x] = PagedOpen{it, walk.last_cta()};
             unsigned odd;
             int row0;  // of the warp
-            if (rows <= 16) {
+            // (what an item's size does not need is not in the kernel: more code costs 8 %)
+            if (M == 16 || rows <= 16) {
                 odd = rows_stay<D, MODE, 1>(a, it, kt0, kt1, part, sh, stages, area, place);
                 row0 = 0;
-            } else if (!WIDE || rows <= 32) {
-                odd = rows_stay<D, MODE, 2>(a, it, kt0, kt1, part, sh, stages, area, place);
+            } else if (M == 32 || rows <= 32) {
+                odd = rows_stay<D, MODE, M >= 32 ? 2 : 1>(a, it, kt0, kt1, part, sh, stages, area, place);
                 row0 = warp % 2 * 16;
             } else {
-                odd = rows_stay<D, MODE, WIDE ? 4 : 2>(a, it, kt0, kt1, part, sh, stages, area, place);
+                odd = rows_stay<D, MODE, M >= 64 ? 4 : 1>(a, it, kt0, kt1, part, sh, stages, area, place);
                 row0 = warp % 4 * 16;
             }
             // rows with a value that is not finite are done again, key by key
@@ -427,30 +428,22 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     }
 }
 
-template <int D, int MODE, bool WIDE>
+template <int D, int MODE>
 static int launch_rows(const PagedArgs &a, const PagedMaps &maps, int ctas, cudaStream_t stream) {
-    auto kernel = paged_rows_kernel<D, MODE, WIDE>;
+    auto kernel = paged_rows_kernel<D, MODE>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(rows_smem<D>())) != cudaSuccess)
         return BD_ERR_LAUNCH;
     return launch_pdl(kernel, dim3(ctas), dim3(kRowsThreads), rows_smem<D>(), stream, a, maps.k, maps.v, maps.heads_outer);
 }
 
-template <int D, int MODE>
-static int launch_rows(const PagedArgs &a, const PagedMaps &maps, bool wide, int ctas, cudaStream_t stream) {
-    if constexpr (MODE != PAGED_F32)  // whose items are always wide
-        if (!wide) return launch_rows<D, MODE, false>(a, maps, ctas, stream);
-    return launch_rows<D, MODE, true>(a, maps, ctas, stream);
-}
-
-int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, bool wide, int ctas,
-                      cudaStream_t stream) {
+int launch_paged_rows(const PagedArgs &a, const PagedMaps &maps, int head_dim, int mode, int ctas, cudaStream_t stream) {
     if (head_dim == 64)
-        return mode == PAGED_F32   ? launch_rows<64, PAGED_F32>(a, maps, wide, ctas, stream)
-               : mode == PAGED_F16 ? launch_rows<64, PAGED_F16>(a, maps, wide, ctas, stream)
-                                   : launch_rows<64, PAGED_BF16>(a, maps, wide, ctas, stream);
-    return mode == PAGED_F32   ? launch_rows<128, PAGED_F32>(a, maps, wide, ctas, stream)
-           : mode == PAGED_F16 ? launch_rows<128, PAGED_F16>(a, maps, wide, ctas, stream)
-                               : launch_rows<128, PAGED_BF16>(a, maps, wide, ctas, stream);
+        return mode == PAGED_F32   ? launch_rows<64, PAGED_F32>(a, maps, ctas, stream)
+               : mode == PAGED_F16 ? launch_rows<64, PAGED_F16>(a, maps, ctas, stream)
+                                   : launch_rows<64, PAGED_BF16>(a, maps, ctas, stream);
+    return mode == PAGED_F32   ? launch_rows<128, PAGED_F32>(a, maps, ctas, stream)
+           : mode == PAGED_F16 ? launch_rows<128, PAGED_F16>(a, maps, ctas, stream)
+                               : launch_rows<128, PAGED_BF16>(a, maps, ctas, stream);
 }
 
 }  // namespace bd

@@ -802,8 +802,9 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
         min(longest, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
         flags.tensor.data_ptr())
-    pairs = requests * kv_heads  # up to 256 of them have one kernel beside the join, whatever their lengths
-    both = dtype is not torch.float32 and pairs > 256 and min(longest, rows) * (heads // kv_heads) > 32
+    # fp16 and bf16 batches of more than 256 (request, kv head) pairs that may hold long requests
+    both = (dtype is not torch.float32 and requests * kv_heads > 256
+            and min(longest, rows) * (heads // kv_heads) > (16 if head_dim == 128 else 32))
     _lib.call("bd_paged_attention", args, _raw_stream(index), kernels=2 + both)
     if own:
         flags.check()
