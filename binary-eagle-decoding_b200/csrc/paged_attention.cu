@@ -164,7 +164,10 @@ static bool cache_map(CUtensorMap *m, const uint16_t *base, const CacheStrides &
     const cuuint32_t each[4] = {1, 1, 1, 1};
     return encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<uint16_t *>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_SWIZZLE_128B,
+                  // a row and no more: with 64 columns 256 bytes are two heads' rows, which other CTAs read
+                  // at other times (131072 keys: 70 us, with 128 bytes 60)
+                  head_dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -425,7 +425,7 @@ constexpr int kTileKeys = 128;
 // Rows of an item in the mma.sync kernel.  For fp16 and bf16 rows also the most that a
 // request has there per kv head; more go to tcgen05 (32 fp16 requests over 4096 keys each,
 // 128 columns: 16 rows take 99 us on mma.sync and 101 on tcgen05, 32 rows 115 and 102; 64
-// requests over 2048 keys, 64 columns: 32 rows 88 and 100).
+// requests over 2048 keys, 64 columns: 32 rows 81 and 100).
 constexpr int kRowsItemMax = 64;
 __host__ __device__ constexpr int rows_item(int head_dim, int mode) {
     return mode == PAGED_F32 ? kRowsItemMax : (head_dim == 64 ? 32 : 16);
@@ -454,8 +454,8 @@ __device__ __forceinline__ bool tile_wait(TileRing &ring, uint64_t *b, uint32_t 
     ring.abort = 1;
     return false;
 }
-__device__ __forceinline__ void tile_arrive(uint64_t *b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+__device__ __forceinline__ void tile_arrive(uint64_t *b, uint32_t count = 1) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
 }
 
 // The places in the ring of a stay's tiles, in order of use.  interleaved: keys and

@@ -8,8 +8,10 @@
 // tile; each has the running maximum, sum and O of its rows over its keys, so the
 // warps meet only at the end of a stay.  S = Q K^T and O += P V are m16n8k16 MMAs.
 // At one token and four heads to a kv head the MMAs, softmax and loads of a warp
-// hide under the 2800 cycles that a tile takes to come from HBM; fp32 rows do twice the
-// MMAs and are bound by them from 64 rows on (24 blocks: 51 % of the MMA pipe).
+// hide under the 2800 cycles that a tile takes to come from HBM: 64 requests over 1024 to
+// 8192 keys (1.09 GB) take 184 us = 5.9 TB/s, one over 131072 keys 94 us = 5.7 TB/s.
+// fp32 rows do twice the MMAs and are bound by these and by the chain through a tile from
+// 64 rows on: 24 draft blocks in a window of 4096 take 177 us, 51 % of the MMA pipe.
 #include "paged_attention.cuh"
 
 namespace bd {
@@ -121,12 +123,19 @@ __device__ __forceinline__ void rows_load_q(const PagedArgs &a, const PagedItem 
 template <int D, int MODE, int RW>
 __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedItem &it, int kt0, int kt1, int part, RowsShared &sh,
                                           uint8_t *stages, uint8_t *area, uint32_t place0) {
-    constexpr int KW = kRowsWarps / RW, KK = kTileKeys / KW;  // key parts, keys of a warp
+    // Parts of the keys; TG groups of them have the tiles in turn, KW parts of KK keys each.
+    // A tile of 64 columns arrives in the time that a warp's chain of waits, MMAs and softmax
+    // takes, so two are worked on at once there (64 tokens of 8 kv heads over 2048 keys:
+    // 70 -> 61 us, 32 rows 87 -> 81).
+    constexpr int TG = D == 64 && RW <= 2 ? 2 : 1, PARTS = kRowsWarps / RW, KW = PARTS / TG, KK = kTileKeys / KW;
     constexpr int kStages = rows_stages<D>();
+    // A group may wait for a stage whose use before belongs to the other group; a barrier
+    // tells two phases apart, so both uses have to be the same group's.
+    static_assert(TG == 1 || kStages / 2 % TG == 0, "stages and groups");
     constexpr bool F32 = MODE == PAGED_F32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3, mi = lane >> 3, r8 = lane & 7;
-    const int rw = warp % RW, kw = warp / RW;
+    const int rw = warp % RW, kp = warp / RW, kw = kp % KW, group = kp / KW;
     rows_load_q<D, MODE>(a, it, area, sh);
     rows_meet();
     const bool live = it.r0 + rw * 16 < it.r1;
@@ -152,7 +161,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
 
-    for (int kt = kt0; kt < kt1; ++kt) {
+    for (int kt = kt0 + group; kt < kt1; kt += TG) {
         const uint32_t pk = place0 + 2 * (kt - kt0), pv = pk + 1, sk = pk % kStages, sv = pv % kStages;
         const uint8_t *ks = stages + sk * tile_bytes<D>();
         uint8_t *vs = stages + sv * tile_bytes<D>();
@@ -197,7 +206,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
             }
         }
         __syncwarp();
-        if (lane == 0) tile_arrive(&sh.ring.empty[sk]);
+        if (lane == 0) tile_arrive(&sh.ring.empty[sk], TG);
         float back[2] = {1.0f, 1.0f};
         if (busy) {
             const bool whole = key0 >= it.lo_all && key0 + KK <= it.hi_all;
@@ -286,7 +295,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
             }
         }
         __syncwarp();
-        if (lane == 0) tile_arrive(&sh.ring.empty[sv]);
+        if (lane == 0) tile_arrive(&sh.ring.empty[sv], TG);
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -295,12 +304,12 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
     }
     // the key parts halve until one is left: the upper half hands its state to the lower
 #pragma unroll
-    for (int half = KW / 2; half >= 1; half >>= 1) {
+    for (int half = PARTS / 2; half >= 1; half >>= 1) {
         rows_meet();  // the area is free: of Q, or of what the last step left
-        const int from = (kw >= half ? kw - half : kw) * RW + rw;  // 0 .. 3
+        const int from = (kp >= half ? kp - half : kp) * RW + rw;  // 0 .. 3
         float *w = reinterpret_cast<float *>(area) + from * 32 * (D / 2) + lane;
         float2 *ml = reinterpret_cast<float2 *>(area + 4 * 32 * (D / 2) * 4) + from * 16 + g;
-        if (kw >= half && kw < 2 * half && live) {
+        if (kp >= half && kp < 2 * half && live) {
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -311,7 +320,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
             }
         }
         rows_meet();
-        if (kw < half && live) {
+        if (kp < half && live) {
             float mine[2], other[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -329,7 +338,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
         }
     }
     unsigned odd_rows = 0;
-    if (kw == 0 && live) {
+    if (kp == 0 && live) {
         bool odd[2] = {false, false};
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
