@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
             set_flag(a.flags, BD_FLAG_NO_PAGES);
         if (b < a.requests) {
             a.owned_out[b] = served || r.need < r.owned ? r.need : r.owned;
-            a.starts[b] = static_cast<int>(row0 + sums.rows - r.count);
+            a.starts[b] = static_cast<int>(min(row0 + sums.rows - r.count, static_cast<int64_t>(INT32_MAX)));
         }
 #pragma unroll 4
         for (int64_t i = tid; i < total.lack; i += n) {

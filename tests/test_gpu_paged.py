@@ -154,6 +154,24 @@ def test_plan_with_too_few_rows_flags_and_stays_inside(ops):
     check_plan(ops, {**many, "rows": 4097})
 
 
+def test_plan_of_more_tokens_than_32_bits_count(ops):
+    """Lengths that each fit and together do not: flagged, and nothing outside the rows is written."""
+    lib = submodule("_lib")
+    requests, width, page, rows = 140_000, 64, 256, 5000
+    table = torch.full((requests, width), -1, dtype=torch.int32, device=DEV)
+    count = torch.full((requests,), width * page, dtype=torch.int32, device=DEV)
+    context, owned = torch.zeros_like(count), torch.zeros_like(count)
+    free, top, flags = torch.arange(70, dtype=torch.int32, device=DEV), dev32([70]), ops.Flags(DEV)
+    plan = ops.page_plan(context, count, table, owned, free, top, page, rows, 70, flags=flags)
+    assert int(flags.tensor.item()) == lib.FLAG_BAD_LENGTH | lib.FLAG_NO_PAGES
+    starts = plan.starts.tolist()
+    assert starts == [min(b * width * page, 2 ** 31 - 1) for b in range(requests + 1)]
+    # the first request has the 64 pages that it needs, from the top of the stack
+    assert table[0].tolist() == list(range(69, 5, -1)) and not (table[1:] >= 0).any() and int(top) == 6
+    assert plan.positions.tolist() == list(range(rows))
+    assert plan.slots.tolist() == [(69 - r // page) * page + r % page for r in range(rows)]
+
+
 @pytest.mark.parametrize("context, count", [([-1, 3], [2, 2]), ([3, 1], [2, -5]), ([60, 1], [5, 1]),
                                             ([2 ** 31 - 1, 1], [2 ** 31 - 1, 1])])
 def test_plan_leaves_out_requests_with_bad_lengths(ops, context, count):
