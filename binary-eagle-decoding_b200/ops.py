@@ -639,13 +639,15 @@ def _cache_shape(k_cache: Tensor, v_cache: Tensor) -> torch.Size:
     return shape
 
 
-def _one_device(index: int, *others: Tensor) -> None:
+def _one_device(index: int, flags: Flags | None, *others: Tensor) -> None:
     """The tensors are on the CUDA device of this index (what ``get_device`` gives)."""
     if index < 0:
         raise ValueError("bitdraft kernels take CUDA tensors")
     for t in others:
         if t.get_device() != index:
             raise ValueError("all tensors must be on one device")
+    if flags is not None and flags.tensor.get_device() != index:
+        raise ValueError("flags must be on the tensors' device")
 
 
 def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free: Tensor, top: Tensor, page_size: int,
@@ -687,7 +689,7 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
     if rows < 0:
         raise ValueError("rows must not be negative")
     index = context.get_device()
-    _one_device(index, count, table, owned, free, top, owned_out, top_out)
+    _one_device(index, flags, count, table, owned, free, top, owned_out, top_out)
     if index != _DEVICE():
         with torch.cuda.device(index):
             return page_plan(context, count, table, owned, free, top, page_size, rows, pool_pages, owned_out, top_out, flags)
@@ -726,7 +728,7 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
     rows = shape[0]
     _int32("slots", slots, (rows,))
     index = k.get_device()
-    _one_device(index, v, slots, k_cache, v_cache)
+    _one_device(index, flags, v, slots, k_cache, v_cache)
     if index != _DEVICE():
         with torch.cuda.device(index):
             return paged_store(k, v, slots, k_cache, v_cache, flags)
@@ -754,8 +756,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
     than ``window`` positions away.  fp32 rows over an fp16 cache (the products keep
     fp32 precision), fp16 over fp16 or bf16 over bf16; head_dim 64 or 128.
     ``longest``: an upper bound of the requests' new tokens, when the caller knows
-    one.  Returns ``out``, whose rows of no request stay as they were; without ``out``
-    a new tensor in which they are zero."""
+    one.  Returns ``out`` (not a part of ``q``), whose rows of no request stay as they
+    were; without ``out`` a new tensor in which they are zero."""
     pages, page_size, kv_heads, cache_dim = _cache_shape(k_cache, v_cache)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or (dtype, k_cache.dtype) not in _ATTENDS:
@@ -781,10 +783,14 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
     elif longest < 1:
         raise ValueError("longest must be at least 1")
     index = q.get_device()
-    _one_device(index, k_cache, v_cache, table, context, starts)
+    _one_device(index, flags, k_cache, v_cache, table, context, starts)
     fresh = out is None
-    if not fresh and (out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous()):
-        raise ValueError("out must be contiguous and like q")
+    if not fresh:
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous():
+            raise ValueError("out must be contiguous and like q")
+        span = ((rows - 1) * q_row + (heads - 1) * q_head + head_dim) * q.element_size()
+        if -out.nbytes < out.data_ptr() - q.data_ptr() < span:
+            raise ValueError("out must not overlap q")
     if index != _DEVICE():
         with torch.cuda.device(index):
             return paged_attention(q, k_cache, v_cache, table, context, starts, causal, window or None, scale, longest or 1,

@@ -422,6 +422,20 @@ def test_attention_out_rows_of_no_request(ops):
     assert ops.paged_attention(batch.q[:0], batch.k, batch.v, batch.table, batch.context, dev32([0, 0, 0])).shape[0] == 0
 
 
+def test_attention_refuses_what_it_cannot_write(ops):
+    """An output over the queries (they are read again for some rows) and flags elsewhere."""
+    batch = Batch([(30, 5), (7, 2)], 4, 2, 64, 16, torch.float16, seed=25)
+    buffer = torch.zeros((2, *batch.q.shape), dtype=torch.float16, device=DEV)
+    buffer[0] = batch.q
+    batch.q = buffer[0]
+    for out in (buffer[0], buffer.flatten()[64:64 + batch.q.numel()].view(batch.q.shape)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            batch.run(ops, out=out)
+    assert torch.equal(batch.run(ops, out=buffer[1]), batch.run(ops))
+    with pytest.raises(ValueError, match="flags must be"):
+        batch.run(ops, flags=ops.Flags(torch.device("cpu")))
+
+
 @pytest.mark.parametrize("row_type", TYPES)
 @pytest.mark.parametrize("count", [5, 90, 300])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
