@@ -9,7 +9,7 @@
 // warps meet only at the end of a stay.  S = Q K^T and O += P V are m16n8k16 MMAs.
 // At one token and four heads to a kv head the MMAs, softmax and loads of a warp
 // hide under the 2800 cycles that a tile takes to come from HBM: 64 requests over 1024 to
-// 8192 keys (1.09 GB) take 184 us = 5.9 TB/s, one over 131072 keys 94 us = 5.7 TB/s.
+// 8192 keys (1.09 GB) take 181 us = 6.0 TB/s, one over 131072 keys 94 us = 5.7 TB/s.
 // fp32 rows do twice the MMAs and are bound by these and by the chain through a tile from
 // 64 rows on: 24 draft blocks in a window of 4096 take 177 us, 51 % of the MMA pipe.
 #include "paged_attention.cuh"

@@ -25,8 +25,8 @@
 // What bounds it: in the steady state the softmax's chain of a step (two 2048-token chunks
 // over 8192 more keys: 575 us = 1075 TFLOP/s; with the softmax left out it would be 1350),
 // and some 10,000 cycles a stay for Q, the first products and the output (over 4096 more
-// keys 345 us = 1000 TFLOP/s, ragged chunks of 64 columns in a window of 1000 keys 50 us).
-// Verification (32 requests of 68 rows over 0.5 to 4 K keys) takes 70 us = 4.0 TB/s.
+// keys 340 us = 1010 TFLOP/s, ragged chunks of 64 columns in a window of 1000 keys 51 us).
+// Verification (32 requests of 68 rows over 0.5 to 4 K keys) takes 64 us = 4.4 TB/s.
 //
 // Every wait is bounded; one that runs out sets BD_FLAG_TIMEOUT and turns the waits
 // that follow into passes, so that all roles walk to their end.
@@ -36,7 +36,10 @@ namespace bd {
 
 constexpr int kTcStep = 64;  // keys of a step of a stream
 constexpr int kTcThreads = 384;
-constexpr int kTcExtra = 3;       // a stay's Q, first and last products and output, in units
+// A stay's Q, first and last products and output, in units: 3 to 4 where a tile has 256 rows, 6
+// to 8 with up to 128 (32 x 17 ragged tokens: 76 us with 3, 74 with 4, 69 with 6, 73 with 8; two
+// 2048-token chunks 244, 235, 234 and 247).
+constexpr int kTcExtra = 6;
 constexpr float kTcSlack = 8.0f;  // growth of a maximum (log2) that leaves O as it is
 
 template <int D>
