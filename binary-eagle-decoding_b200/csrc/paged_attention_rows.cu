@@ -9,16 +9,22 @@
 // warps meet only at the end of a stay.  S = Q K^T and O += P V are m16n8k16 MMAs.
 // At one token and four heads to a kv head the MMAs, softmax and loads of a warp
 // hide under the 2800 cycles that a tile takes to come from HBM: 64 requests over 1024 to
-// 8192 keys (1.09 GB) take 181 us = 6.0 TB/s, one over 131072 keys 94 us = 5.7 TB/s.
+// 8192 keys (1.09 GB) take 171 us = 6.4 TB/s, one over 131072 keys 94 us = 5.7 TB/s.
 // fp32 rows do twice the MMAs and are bound by these and by the chain through a tile from
-// 64 rows on: 24 draft blocks in a window of 4096 take 177 us, 51 % of the MMA pipe.
+// 64 rows on: 24 draft blocks in a window of 4096 take 172 us, 53 % of the MMA pipe.
 #include "paged_attention.cuh"
 
 namespace bd {
 
 constexpr int kRowsWarps = 8;
 constexpr int kPlane = 64;  // rows of a plane of Q in shared memory
-constexpr int kRowsExtra = 1;  // a stay's Q, joining and output, in units
+// A stay's Q, joining and output, in units; the tiles of fp32 rows of 128 columns take longer
+// (64 ragged tokens: 197 us with 1, 185 with 2, 184 with 4, of 64 columns 127, 119 and 112; 24
+// draft blocks 164, 157 and 160).
+template <int D, int MODE>
+constexpr int rows_extra() {
+    return MODE == PAGED_F32 && D == 128 ? 2 : 4;
+}
 constexpr int kRowsThreads = 384;
 
 template <int D>
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     grid_wait();
     grid_launch_dependents();
     constexpr int M = rows_item(D, MODE);
-    PagedWalk<M, kTileKeys, kRowsExtra, false> walk;
+    PagedWalk<M, kTileKeys, rows_extra<D, MODE>(), false> walk;
     if (tid == 0) a.parts[0].open[blockIdx.x].last = -1;
     if (!walk.begin(a, sh.walk, blockIdx.x, gridDim.x)) return;
     // registers: 384 x 168 at launch = 128 x 56 + 256 x 224
