@@ -9,9 +9,11 @@
 // One pass over the keys with a running maximum and sum per row, S = Q K^T and
 // O = P V on the tensor cores with fp32 accumulators.  fp32 queries (over an fp16
 // cache) enter as fp16 hi + lo halves of the row over a power of two, and P as hi +
-// lo halves, which keeps about 22 bits of each.  fp16 and bf16 rows round P once to
-// the cache's type (relative 2^-11 and 2^-8 at most, the size of the output's own
-// rounding); the row sum adds the fp32 values.
+// lo halves.  fp16 and bf16 rows round P once to the cache's type (relative 2^-11 and 2^-8 at
+// most, the size of the output's own rounding); the row sum adds the fp32 values.  fp16 has
+// no step under 2^-24, so P is scaled up to 2^15 there: halves keep 22 bits of weights down to
+// 2^-18 of the row's largest and an error of 2^-40 of it below; a rounded P its 2^-11 down to
+// 2^-29 (tcgen05: 2^-25) and an error of 2^-40 (2^-36) below.
 //
 // Two kernels: requests of up to 16 rows per kv head (32 with 64 columns), and fp32 rows of
 // any count, run on mma.sync (paged_attention_rows.cu), the others on tcgen05

@@ -74,6 +74,14 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// The weights of fp16 caches enter the products times 2^15 (at most 32768), which leaves fp16's whole
+// range below them: unscaled, every weight under 2^-25 of the largest was lost to O and not to
+// the sum (8192 keys 18 nats below one of small value: up to a third of the output).
+template <int MODE>
+constexpr float rows_weight_scale() {
+    return MODE == PAGED_BF16 ? 1.0f : 32768.0f;
+}
+
 __device__ __forceinline__ void rows_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // The Q rows of an item into shared memory, four threads to a row.  fp32 rows over the
@@ -139,6 +147,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
     // tells two phases apart, so both uses have to be the same group's.
     static_assert(TG == 1 || kStages / 2 % TG == 0, "stages and groups");
     constexpr bool F32 = MODE == PAGED_F32;
+    constexpr float kScale = rows_weight_scale<MODE>();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3, mi = lane >> 3, r8 = lane & 7;
     const int rw = warp % RW, kp = warp / RW, kw = kp % KW, group = kp / KW;
@@ -262,7 +271,8 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
             for (int k = 0; k < KK / 16; ++k)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float x = s[2 * k + (j >> 1)][2 * (j & 1)], y = s[2 * k + (j >> 1)][2 * (j & 1) + 1];
+                    const float x = s[2 * k + (j >> 1)][2 * (j & 1)] * kScale;
+                    const float y = s[2 * k + (j >> 1)][2 * (j & 1) + 1] * kScale;
                     if (F32)
                         split_half2(x, y, ph[k][j], pl[F32 ? k : 0][j]);
                     else
@@ -308,6 +318,11 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
+    if (MODE != PAGED_BF16)
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= 1.0f / kScale;
     // the key parts halve until one is left: the upper half hands its state to the lower
 #pragma unroll
     for (int half = PARTS / 2; half >= 1; half >>= 1) {

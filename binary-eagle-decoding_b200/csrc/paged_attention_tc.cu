@@ -15,9 +15,9 @@
 // softmax, P V of a stream left the tensor pipe 55 % idle (8192 + 2048 keys: 681 us).
 // Warps 0-3 and 4-7 are the softmax of stream 0 and 1, a thread to a row: S from
 // TMEM, running maximum and sum, P as 16-bit values back over S's columns.  O stays
-// in TMEM; a row's O is rescaled only when its maximum has grown by more than 2^8
-// since the last time (P is at most 2^8 then, the sum and O scale alike), which
-// takes the rescaling off the usual path.  Warps 10 and 11 load key and value tiles by TMA
+// in TMEM; a row's O is rescaled only when its maximum has grown by more than 2^8 (fp16
+// rows 2^4) since the last time (the sum and O scale alike), which takes the rescaling off the
+// usual path.  Warps 10 and 11 load key and value tiles by TMA
 // (a box per page piece and 64 columns) into one ring in the order of their use;
 // warps 8 and 9 issue, each for a stream, S = Q K^T (both operands in shared memory)
 // and O += P V (P in TMEM, V as it lies, its rows being the reduction).
@@ -40,7 +40,23 @@ constexpr int kTcThreads = 384;
 // to 8 with up to 128 (32 x 17 ragged tokens: 76 us with 3, 74 with 4, 69 with 6, 73 with 8; two
 // 2048-token chunks 244, 235, 234 and 247).
 constexpr int kTcExtra = 6;
-constexpr float kTcSlack = 8.0f;  // growth of a maximum (log2) that leaves O as it is
+// A row's weights are 2^(x - base), with the base kTcShift below its maximum as it was at the last
+// rescaling; growth of the maximum by up to kTcSlack leaves base and O as they are.  For fp16
+// the two add up to 2^15, so that weights down to 2^-36 of the largest are held (with a shift of
+// 0 and a slack of 8, those under 2^-25 were lost to O and not to the sum); bf16 has fp32's range.
+template <int MODE>
+constexpr float tc_shift() {
+    return MODE == PAGED_F16 ? 11.0f : 0.0f;
+}
+template <int MODE>
+constexpr float tc_slack() {
+    return MODE == PAGED_F16 ? 4.0f : 8.0f;
+}
+// The base of a maximum; from 2^20 on, where its own steps are larger than a sixteenth, without the shift.
+template <int MODE>
+__device__ __forceinline__ float tc_base(float m) {
+    return m == -INFINITY ? 0.0f : (fabsf(m) < 1048576.0f ? m - tc_shift<MODE>() : m);
+}
 
 template <int D>
 constexpr int tc_stages() {
@@ -393,7 +409,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             if (lane == 0) tile_arrive(&sh.q_full);
 
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, base = 0.0f, l = 0.0f;
             for (int i = 0; i < count; ++i) {
                 const int buffer = i & 1;
                 const uint32_t at = s_at + buffer * kTcStep;
@@ -422,12 +438,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int k = 2; k < 16; k += 2) top[x] = max3(top[x], v[k], v[k + 1]);
                     }
                     const float now = fmaxf(max3(top[0], top[1], top[2]), top[3]) * c;
-                    const bool grows = now > m + kTcSlack || m == -INFINITY;
+                    const bool grows = now > m + tc_slack<MODE>() || m == -INFINITY;
                     if (__any_sync(0xffffffffu, grows && m != -INFINITY)) {
                         // the products so far are in O (this S says so of all but the last step's)
                         tile_wait(sh.ring, &sh.o_step[t][buffer ^ 1], steps[buffer ^ 1] - 1);
                         tc_fence_after();
-                        const float back = grows ? exp2_fast(m - now) : 1.0f;
+                        const float back = grows ? exp2_fast(base - tc_base<MODE>(now)) : 1.0f;
                         l *= m == -INFINITY ? 1.0f : back;
 #pragma unroll 1
                         for (int x = 0; x < D / 16; ++x) {
@@ -439,8 +455,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             tc_st16(o_at + 16 * x, o);
                         }
                     }
-                    if (grows) m = now;
-                    const float base = m == -INFINITY ? 0.0f : m;
+                    if (grows) {
+                        m = now;
+                        base = tc_base<MODE>(now);
+                    }
                     const float2 c2 = make_float2(c, c), base2 = make_float2(-base, -base);
                     float2 sum[4];
                     uint32_t w[32];
@@ -463,6 +481,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             tile_wait(sh.ring, &sh.o_full[t], stays++);
             tc_fence_after();
+            if (m != -INFINITY) m = base;  // what l and O are relative to
             float4 *swap = reinterpret_cast<float4 *>(sq);  // Q is done with: O of stream 1, [column / 4][row]
             float mine_w = 1.0f, other_w = 0.0f;
             if (!both) {
@@ -482,7 +501,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (t == 0 && warp_live) {
                     const float2 x = sh.ml[lrow];
-                    const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
+                    const float top = fmaxf(m, x.x);
+                    base = top == -INFINITY ? 0.0f : top;
                     mine_w = exp2_fast(m - base);
                     other_w = exp2_fast(x.x - base);
                     l = l * mine_w + x.y * other_w;

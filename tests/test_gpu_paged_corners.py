@@ -1,0 +1,89 @@
+"""Corners of the paged cache on the GPU: small weights beside a large one, values at the
+types' limits, values that are not finite, lengths that do not fit (needs a B200)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from conftest import package, submodule
+from test_gpu_paged import DEV, HALF_STEP, TYPES, Batch, dev32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return package().ops
+
+
+# ------------------------------------------------------------------ small weights
+
+
+def exact(batch, scale=None, window=None):
+    """Causal attention in 64 bits: (output, sum of weight x |v|, largest weight, sum of |q k|
+    x scale at its largest), per row and head."""
+    scale = batch.head_dim ** -0.5 if scale is None else scale
+    group, row = batch.heads // batch.kv_heads, 0
+    out = torch.zeros(batch.q.shape, dtype=torch.float64, device=DEV)
+    size, peak, reach = torch.zeros_like(out), torch.zeros_like(out), torch.zeros_like(out)
+    for b, (context, count) in enumerate(batch.lengths):
+        at = torch.arange(context + count, device=DEV)
+        page = batch.table[b, at // batch.page].long()
+        k, v = batch.k[page, at % batch.page].double(), batch.v[page, at % batch.page].double()
+        gap = (context + torch.arange(count, device=DEV))[:, None] - at
+        hidden = (gap < 0) | (gap >= (window or 2 ** 40))
+        here = slice(row, row + count)
+        for h in range(batch.heads):
+            q, kh, vh = batch.q[here, h].double(), k[:, h // group], v[:, h // group]
+            p = torch.softmax((q @ kh.T * scale).masked_fill(hidden, -math.inf), -1)
+            out[here, h], size[here, h] = p @ vh, p @ vh.abs()
+            peak[here, h] = p.amax(-1, keepdim=True)
+            reach[here, h] = (q.abs() @ kh.abs().T * abs(scale)).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+        row += count
+    return out, size, peak, reach
+
+
+def small_weights_bound(batch, out, size, peak, reach):
+    """Error of the weights and sums.  The exponent: head_dim products added in fp32, the scale,
+    log2 e and the maximum's subtraction rounded, ex2 within 2^-22, and for fp32 rows the
+    halves' 2^-21 each of a product.  A weight's rounding: 2^-21 for fp32 rows, half a step of
+    the cache's type for others; where that type is fp16, at most half its smallest step, 2^-25,
+    of weights scaled so that the largest is 2^11 or more (fp32 rows 2^15): 2^-36 (2^-40) of the
+    largest, a key.
+    Sums of length / 16 + 64 steps in fp32, and the output's rounding."""
+    u, d, f32 = HALF_STEP[batch.q.dtype], batch.head_dim, batch.q.dtype == torch.float32
+    length = max(a + b for a, b in batch.lengths)
+    delta = (d + 12) * 2.0 ** -23 * reach + 2.0 ** -21 + (2.0 ** -20 * reach if f32 else 0.0)
+    sums = 2 * (length / 16 + 64) * 2.0 ** -23
+    step = {torch.float32: 2.0 ** -40, torch.float16: 2.0 ** -36, torch.bfloat16: 0.0}[batch.q.dtype]
+    lost = length * step * peak * batch.v.abs().amax().double()
+    return u * out.abs() + size * ((2.0 ** -21 if f32 else u) + 2 * delta + sums) * 1.1 + lost
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("requests, keys, count, head_dim", [(160, 8192, 1, 128), (160, 8192, 1, 64), (80, 16384, 20, 128),
+                                                             (80, 16384, 40, 64), (2, 100_000, 20, 128)])
+@pytest.mark.parametrize("nats", [11.0, 15.0, 18.5])
+def test_many_small_weights_beside_a_large_one(ops, row_type, requests, keys, count, head_dim, nats):
+    """A first key that draws nearly all of a row's weight and holds little, the others each
+    `nats` below it: together they are the output.  With 80 and more pairs an item
+    stays whole in one CTA and one running maximum."""
+    kv_heads = 2 if requests == 80 else 1
+    batch = Batch([(keys - count, count)] * requests, kv_heads, kv_heads, head_dim, 64, row_type, seed=int(nats))
+    q = batch.q.clone() * 0.05
+    q[..., 0] = 8.0
+    batch.q = q
+    batch.k.mul_(0.05)
+    batch.k[..., 0] = 0.0
+    batch.v.add_(0.5)
+    first = batch.table[:, 0].long()
+    batch.k[first, 0] = 0.0
+    batch.k[first, 0, :, 0] = nats * head_dim ** 0.5 / 8.0
+    batch.v[first, 0] = 0.0
+    want, *how = exact(batch)
+    err = (batch.run(ops).double() - want).abs()
+    bound = small_weights_bound(batch, want, *how)
+    assert bool((err <= bound).all()), (float((err / bound).max()), float(err.norm() / want.norm()))
