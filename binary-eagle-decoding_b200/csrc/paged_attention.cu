@@ -8,7 +8,7 @@
 //
 // One pass over the keys with a running maximum and sum per row, S = Q K^T and
 // O = P V on the tensor cores with fp32 accumulators.  fp32 queries (over an fp16
-// cache) enter as fp16 hi + lo halves of the row over a power of two, and P as hi +
+// cache) enter as fp16 hi + lo halves of the row times a power of two, and P as hi +
 // lo halves.  fp16 and bf16 rows round P once to the cache's type (relative 2^-11 and 2^-8 at
 // most, the size of the output's own rounding); the row sum adds the fp32 values.  fp16 has
 // no step under 2^-24, so P is scaled up to 2^15 there: halves keep 22 bits of weights down to

@@ -84,9 +84,11 @@ constexpr float rows_weight_scale() {
 
 __device__ __forceinline__ void rows_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// The Q rows of an item into shared memory, four threads to a row.  fp32 rows over the
-// row's power of two, so that the halves of values up to 1 lose nothing to fp16's
-// range; fold = scale x log2 e x that power.
+// The Q rows of an item into shared memory, four threads to a row.  fp32 rows are scaled by a
+// power of two that takes the row's largest value to 2^14 .. 2^15, fp16's upper end, so that
+// the halves hold values down to 2^-17 of the largest with 22 bits and smaller ones within
+// 2^-39 of it (scaled to 1, a row's values under 2^-25 of its largest were 0); fold = scale x
+// log2 e over that power.
 template <int D, int MODE>
 __device__ __forceinline__ void rows_load_q(const PagedArgs &a, const PagedItem &it, uint8_t *area, RowsShared &sh) {
     constexpr int kChunks = D / 32;  // 16-byte pieces (of 16-bit values) of a thread
@@ -106,7 +108,7 @@ __device__ __forceinline__ void rows_load_q(const PagedArgs &a, const PagedItem 
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         int e = 0;
-        if (big > 0.0f && big < INFINITY) e = min(max(ilogbf(big) + 1, -100), 126);
+        if (big > 0.0f && big < INFINITY) e = max(ilogbf(big) + 1, -100) - 15;
         const float down = ldexpf(1.0f, -e);
         if (part == 0) sh.fold[r] = a.scale_log2 * ldexpf(1.0f, e);
 #pragma unroll

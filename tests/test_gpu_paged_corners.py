@@ -87,3 +87,23 @@ def test_many_small_weights_beside_a_large_one(ops, row_type, requests, keys, co
     err = (batch.run(ops).double() - want).abs()
     bound = small_weights_bound(batch, want, *how)
     assert bool((err <= bound).all()), (float((err / bound).max()), float(err.norm() / want.norm()))
+
+
+@pytest.mark.parametrize("count, head_dim", [(1, 128), (16, 128), (70, 64)])
+@pytest.mark.parametrize("big", [1e3, 1e5, 1e6, 3e38])
+def test_fp32_rows_with_one_large_value(ops, count, head_dim, big):
+    """The keys hold nothing where the rows are large, so the rows' small values decide.  A value's
+    halves are off by 2^-22 of it or by half of fp16's smallest step, at the row's largest value
+    scaled to 2^14 or more: 2^-25 / 2^14 of that value, on each of the row's products."""
+    batch = Batch([(300, count), (40, 2)], 4, 2, head_dim, 16, torch.float32, seed=31)
+    q = batch.q.clone()
+    q[..., 5] = big
+    batch.q = q
+    batch.k[..., 5] = 0.0
+    want, size, peak, reach = exact(batch)
+    err = (batch.run(ops).double() - want).abs()
+    halves = 2.0 ** -39 * big * batch.k.double().abs().sum(-1).amax() * head_dim ** -0.5
+    if big > 1e30:  # their products are all lost: only the mean over the keys of flat weights is left
+        assert bool(torch.isfinite(err).all())
+    else:
+        assert bool((err <= small_weights_bound(batch, want, size, peak, reach) + 2.2 * halves * size).all())
