@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
                 }
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = 1.0f / l;  // l is 0 only when every seen score is -inf: not a number
         const int64_t at = paged_row_offset(a, it, row, a.out_row, D) + lane * V;
         float probe = 0.0f;
 #pragma unroll

@@ -387,7 +387,7 @@ __device__ __forceinline__ void paged_slow_row(const PagedArgs &a, const PagedIt
     const int64_t at = paged_row_offset(a, it, row, a.out_row, D) + lane * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float y = l == 0.0f ? 0.0f : o[i] / l;
+        const float y = o[i] / l;
         if (MODE == PAGED_F32)
             static_cast<float *>(a.out)[at + i] = y;
         else if (MODE == PAGED_BF16)

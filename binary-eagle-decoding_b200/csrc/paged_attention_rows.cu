@@ -376,7 +376,7 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
                 if (t == 0) *reinterpret_cast<float2 *>(a.parts[0].ml + at * 2) = make_float2(m[r], l[r]);
                 continue;
             }
-            const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+            const float inv = 1.0f / l[r];
             const int64_t at = paged_row_offset(a, it, row, a.out_row, D);
             float probe = 0.0f;
 #pragma unroll

@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
             if ((both || t == 0) && warp_live) {
-                const float inv = out >= 0 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+                const float inv = out >= 0 ? 1.0f : 1.0f / l;
                 float probe = 0.0f;
                 const int64_t part_row = static_cast<int64_t>(max(out, 0)) * kTcItem + row - it.r0;
                 const int64_t at = live ? paged_row_offset(a, it, row, a.out_row, D) : 0;

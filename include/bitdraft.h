@@ -469,6 +469,7 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * (BD_FLAG_BAD_LENGTH); keys on a page outside the pool count as zeros
  * (BD_FLAG_BAD_PAGE); entries of pages that no token sees are not read.  What the
  * cache holds at keys that a row does not see never reaches it, not even as NaN:
+ * a row whose own scores are all -infinity is not a number, as its softmax is;
  * a row with a value that is not finite is done again over its own keys, by one warp
  * and so slowly (about 0.3 us a key).  Strides as at bd_paged_store; caches are read
  * by TMA, so strides that a tensor map cannot hold are BD_ERR_ALIGNMENT too.

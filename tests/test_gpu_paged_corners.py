@@ -107,3 +107,46 @@ def test_fp32_rows_with_one_large_value(ops, count, head_dim, big):
         assert bool(torch.isfinite(err).all())
     else:
         assert bool((err <= small_weights_bound(batch, want, size, peak, reach) + 2.2 * halves * size).all())
+
+
+# ------------------------------------------------------------------ values that are not finite
+
+
+def matches_exact(ops, batch, **how):
+    """Finite where the definition is, within the bound, and not a number where it is not."""
+    got, (want, *rest) = batch.run(ops, **how).double(), exact(batch)
+    real = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isfinite(got), real)
+    bound = torch.nan_to_num(small_weights_bound(batch, *(torch.nan_to_num(x, posinf=1.0, neginf=1.0) for x in (want, *rest))))
+    assert bool(((got - want).abs() <= bound)[real].all())
+    return real
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("count, head_dim", [(1, 128), (5, 64), (20, 128), (90, 64), (300, 128)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_keys_that_are_not_finite(ops, row_type, count, head_dim, value):
+    """A key of a later token must not reach earlier ones; where it is seen, a score of -inf
+    only removes the key and one of +inf or NaN leaves no number."""
+    batch = Batch([(150, count), (0, 1), (70, 2)], 4, 2, head_dim, 16, row_type, seed=41)
+    spot = 150 + count // 2
+    batch.k[batch.table[0, spot // 16].long(), spot % 16, 1, 3] = value
+    batch.k[batch.table[2, 0].long(), 7, 0, 0] = value  # key 7 of the last request
+    real = matches_exact(ops, batch)
+    assert bool(real[:count // 2].all()) and bool(real[:, :2][:count + 1].all())
+    if math.isnan(value):
+        assert not bool(real[count // 2:count, 2:].any())
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("count, head_dim", [(1, 128), (3, 64), (20, 128), (90, 64)])
+def test_a_row_whose_scores_are_all_minus_infinity_is_not_a_number(ops, row_type, count, head_dim):
+    """As the softmax of its definition is, split over CTAs or not."""
+    batch = Batch([(0, count), (700, 2)], 4, 2, head_dim, 16, row_type, seed=42)
+    q = batch.q.clone()
+    q[:count, :, 0] = 2.0
+    batch.q = q
+    length = torch.arange(count, device=DEV)
+    batch.k[batch.table[0, length // 16].long(), length % 16, 0, 0] = -math.inf
+    real = matches_exact(ops, batch)
+    assert not bool(real[:count, :2].any()) and bool(real[:count, 2:].all()) and bool(real[count:].all())
