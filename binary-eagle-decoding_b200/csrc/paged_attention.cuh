@@ -345,8 +345,9 @@ struct PagedWalk {
 
 // One row by one warp, key by key: for rows whose tile products met values that are
 // not finite.  There a masked key's infinity or NaN times the zero of its weight
-// would reach the row, so only keys that the row sees are touched here.  0.3 us a key;
-// four keys at once were 1.4 times as fast, and their code made the others 2 % slower.
+// would reach the row, so only keys that the row sees are touched here.  0.3 us a key, 0.85
+// when all warps of an SM do rows of 200,000 keys; four keys at once were 1.4 times as fast, and
+// their code made the others 2 % slower.
 template <int D, int MODE>
 __device__ __forceinline__ void paged_slow_row(const PagedArgs &a, const PagedItem &it, int row) {
     constexpr int V = D / 32;
@@ -433,8 +434,9 @@ __host__ __device__ constexpr int rows_item(int head_dim, int mode) {
 }
 constexpr int kTcItem = 256;  // tcgen05 kernel: two streams of 128
 constexpr int kMaxStages = 8;
-// Limit of a wait.  The longest that is in order is behind 32 rows done key by key, 0.3 us a
-// key: 0.4 s at 32000 keys passed with 2^21 polls, this is for four times as many.
+// Limit of a wait, more than a second.  Those in order are for the work on a tile or for the begin
+// or end of a stay, microseconds at any length, or for rows that are done key by key, which
+// may take long and are not counted (TileRing::slow).
 constexpr uint32_t kTilePolls = 1u << 23;
 
 template <int D>
@@ -445,17 +447,29 @@ constexpr int tile_bytes() {
 struct TileRing {
     uint64_t full[kMaxStages], empty[kMaxStages];
     volatile int abort;
+    int slow;  // warps that do rows key by key
 };
 
 // Waits for phase `count` (0, 1, ..) of a barrier.  A wait that runs out sets `abort`,
-// after which all waits pass: every role walks to its end.
+// after which all waits pass: every role walks to its end.  Polls count only while no warp
+// does rows key by key: that work ends by itself, but after a time that grows with the keys.
 __device__ __forceinline__ bool tile_wait(TileRing &ring, uint64_t *b, uint32_t count) {
     for (uint32_t i = 0; i < kTilePolls; ++i) {
         if (mbar_try_wait(b, count & 1)) return true;
         if (ring.abort) return false;
+        if (*const_cast<volatile int *>(&ring.slow)) i = 0;
     }
     ring.abort = 1;
     return false;
+}
+// The rows of a stay (bit i: row0 + i) whose values are not finite, again, by the warp that did them.
+template <int D, int MODE>
+__device__ __forceinline__ void slow_rows(const PagedArgs &a, const PagedItem &it, TileRing &ring, int row0, unsigned odd) {
+    if (!odd) return;
+    const bool leader = (threadIdx.x & 31) == 0;
+    if (leader) atomicAdd(&ring.slow, 1);
+    for (; odd; odd &= odd - 1) paged_slow_row<D, MODE>(a, it, row0 + __ffs(odd) - 1);
+    if (leader) atomicSub(&ring.slow, 1);
 }
 __device__ __forceinline__ void tile_arrive(uint64_t *b, uint32_t count = 1) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");

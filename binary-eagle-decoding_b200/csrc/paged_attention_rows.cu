@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             mbar_init(&sh.ring.full[s], 1);
             mbar_init(&sh.ring.empty[s], kRowsWarps);
         }
-        sh.ring.abort = 0;
+        sh.ring.abort = sh.ring.slow = 0;
         mbar_init_fence();
     }
     __syncthreads();
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             }
             // rows with a value that is not finite are done again, key by key
             __syncwarp();
-            for (; odd; odd &= odd - 1) paged_slow_row<D, MODE>(a, it, it.r0 + row0 + __ffs(odd) - 1);
+            slow_rows<D, MODE>(a, it, sh.ring, it.r0 + row0, odd);
             rows_meet();  // the area is free for the next Q
             place += 2 * (kt1 - kt0);
         }

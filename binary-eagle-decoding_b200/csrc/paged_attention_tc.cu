@@ -182,6 +182,7 @@ __device__ __forceinline__ bool tc_wait(TileRing &ring, uint64_t *b, uint32_t co
     for (uint32_t i = 0; i < kTilePolls; ++i) {
         if (__any_sync(0xffffffffu, mbar_try_wait(b, count & 1))) return true;
         if (__any_sync(0xffffffffu, ring.abort)) return false;
+        if (__any_sync(0xffffffffu, *const_cast<volatile int *>(&ring.slow))) i = 0;
     }
     ring.abort = 1;
     return false;
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&sh.o_full[t], 1);
             mbar_init(&sh.drain[t], 1);
         }
-        sh.ring.abort = 0;
+        sh.ring.abort = sh.ring.slow = 0;
         mbar_init_fence();
     }
     if (warp == 9) {
@@ -580,12 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 if (out >= 0 && live) *reinterpret_cast<float2 *>(a.parts[1].ml + part_row * 2) = make_float2(m, l);
                 // rows with a value that is not finite are done again, key by key
-                unsigned odd = __ballot_sync(0xffffffffu, live && out < 0 && !(probe == 0.0f));
-                while (odd) {
-                    const int r = __ffs(odd) - 1;
-                    odd &= odd - 1;
-                    paged_slow_row<D, MODE>(a, it, row - lane + r);
-                }
+                slow_rows<D, MODE>(a, it, sh.ring, row - lane, __ballot_sync(0xffffffffu, live && out < 0 && !(probe == 0.0f)));
             }
             tc_fence_before();
             if (!both) asm volatile("bar.sync 1, 256;" ::: "memory");  // the swap area is free

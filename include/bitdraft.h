@@ -471,7 +471,7 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * cache holds at keys that a row does not see never reaches it, not even as NaN:
  * a row whose own scores are all -infinity is not a number, as its softmax is;
  * a row with a value that is not finite is done again over its own keys, by one warp
- * and so slowly (about 0.3 us a key).  Strides as at bd_paged_store; caches are read
+ * and so slowly (0.3 to 0.9 us a key; the waits of its SM allow for it).  Strides as at bd_paged_store; caches are read
  * by TMA, so strides that a tensor map cannot hold are BD_ERR_ALIGNMENT too.
  * The workspace needs no clearing; calls that overlap on the GPU need their own.
  * Results do not depend on what else the GPU runs: partials are joined in order. */

@@ -150,3 +150,23 @@ def test_a_row_whose_scores_are_all_minus_infinity_is_not_a_number(ops, row_type
     batch.k[batch.table[0, length // 16].long(), length % 16, 0, 0] = -math.inf
     real = matches_exact(ops, batch)
     assert not bool(real[:count, :2].any()) and bool(real[:count, 2:].all()) and bool(real[count:].all())
+
+
+@pytest.mark.parametrize("row_type, count, keys", [(torch.float32, 64, 250_000), (torch.float16, 256, 200_000),
+                                                   (torch.bfloat16, 256, 200_000), (torch.float16, 3, 20_000)])
+def test_a_request_that_is_not_finite_spoils_no_other(ops, row_type, count, keys):
+    """All rows of a request are not numbers, over more keys than a wait of the kernels lasts when
+    they are done one by one; the requests share their pages and all but those rows stay as they were."""
+    requests, page = 160, 256
+    batch = Batch([(keys - count, count)], 1, 1, 64, page, row_type, seed=43)
+    table = batch.table.expand(requests, -1).contiguous()
+    context = batch.context.expand(requests).contiguous()
+    starts = torch.arange(requests + 1, dtype=torch.int32, device=DEV) * count
+    q = torch.randn((requests * count, 1, 64), device=DEV).to(row_type)
+    flags = ops.Flags(DEV)
+    want = ops.paged_attention(q, batch.k, batch.v, table, context, starts, flags=flags)
+    q[:count, 0, 9] = math.nan  # this request is whole in the first CTA
+    got = ops.paged_attention(q, batch.k, batch.v, table, context, starts, flags=flags)
+    flags.check()
+    assert torch.equal(got[count:], want[count:])
+    assert bool(torch.isnan(got[:count]).all()) and bool(torch.isfinite(want).all())
