@@ -462,6 +462,17 @@ __device__ __forceinline__ bool tile_wait(TileRing &ring, uint64_t *b, uint32_t 
     ring.abort = 1;
     return false;
 }
+// tile_wait() by a whole warp, in branches that are the same for all lanes.
+__device__ __forceinline__ bool warp_wait(TileRing &ring, uint64_t *b, uint32_t count) {
+    for (uint32_t i = 0; i < kTilePolls; ++i) {
+        if (__any_sync(0xffffffffu, mbar_try_wait(b, count & 1))) return true;
+        if (__any_sync(0xffffffffu, ring.abort)) return false;
+        if (__any_sync(0xffffffffu, *const_cast<volatile int *>(&ring.slow))) i = 0;
+    }
+    ring.abort = 1;
+    return false;
+}
+
 // The rows of a stay (bit i: row0 + i) whose values are not finite, again, by the warp that did them.
 template <int D, int MODE>
 __device__ __forceinline__ void slow_rows(const PagedArgs &a, const PagedItem &it, TileRing &ring, int row0, unsigned odd) {
@@ -494,8 +505,8 @@ struct PagedMaps {
 
 // The whole run of loading warp `turn` of LOADERS, which have the tiles in turn: a warp
 // issues the boxes of its lanes one after the other (about 130 cycles each), which at
-// pages of 16 keys is longer than a tile takes to arrive.  A piece without a key that some row sees, or on a page
-// outside the pool, is read as zeros (a box behind the last page).
+// pages of 16 keys is longer than a tile takes to arrive.  A piece without a key that some
+// row sees, or on a page outside the pool, is read as zeros (a box behind the last page).
 template <int D, int STAGES, int LOADERS, typename Walk>
 __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileRing &ring, uint8_t *stages,
                                            const CUtensorMap *k_map, const CUtensorMap *v_map, int heads_outer,
@@ -506,6 +517,11 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
     const int pieces = kTileKeys / piece;
     const int block = lane / pieces, part = lane - block * pieces;
     uint32_t place = 0;
+    // The copies of this warp in a range of places land before the CTA may end.
+    auto land = [&](uint32_t from, uint32_t to, uint32_t polls) {
+        for (uint32_t j = from; j < to; ++j)
+            if (j % LOADERS == turn) mbar_wait_bounded(&ring.full[j % STAGES], (j / STAGES) & 1, polls);
+    };
     PagedItem it;
     int kt0, kt1, out;
     while (walk.next(a, it, kt0, kt1, out)) {
@@ -520,8 +536,14 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
             const bool seen = block < D / 64 && key < it.hi && key + piece > it.lo;
             int page = seen ? __ldg(table + (key >> a.page_shift)) : -1;
             const uint32_t s = place % STAGES;
-            if (place >= STAGES) tile_wait(ring, &ring.empty[s], place / STAGES - 1);
-            if (ring.abort) continue;
+            // After a wait ran out, stages are released before their tiles have come, so no further
+            // copy may start; all lanes decide alike, since a stage's boxes are one transaction.
+            if ((place >= STAGES && !warp_wait(ring, &ring.empty[s], place / STAGES - 1)) ||
+                __any_sync(0xffffffffu, ring.abort)) {
+                // this warp's copies may be one turn behind the ring's last STAGES places
+                land(place > STAGES + LOADERS ? place - STAGES - LOADERS : 0, place, 1u << 16);
+                return;
+            }
             if (lane == 0) mbar_expect_tx(&ring.full[s], tile_bytes<D>());
             __syncwarp();
             if (block < D / 64) {
@@ -540,10 +562,8 @@ __device__ __forceinline__ void load_tiles(const PagedArgs &a, Walk &walk, TileR
             __syncwarp();
         }
     }
-    // after a wait ran out: the copies in flight land before the CTA ends
-    if (ring.abort)
-        for (uint32_t j = place > STAGES ? place - STAGES : 0; j < place; ++j)
-            if (j % LOADERS == turn) mbar_wait_bounded(&ring.full[j % STAGES], (j / STAGES) & 1, kTilePolls);
+    // the last use of every stage (whoever reads these tiles waits for them too, but for a wait that ran out)
+    land(place > STAGES ? place - STAGES : 0, place, kTilePolls);
 }
 
 // ------------------------------------------------------------------ launches

@@ -177,17 +177,6 @@ __device__ __forceinline__ uint32_t tc_elect() {
 // A value that is the same in all lanes, as one the compiler knows to be: a reduction
 // over the warp leaves its result in a uniform register.
 __device__ __forceinline__ uint32_t tc_uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
-// tile_wait() by a whole warp, in branches that are the same for all lanes.
-__device__ __forceinline__ bool tc_wait(TileRing &ring, uint64_t *b, uint32_t count) {
-    for (uint32_t i = 0; i < kTilePolls; ++i) {
-        if (__any_sync(0xffffffffu, mbar_try_wait(b, count & 1))) return true;
-        if (__any_sync(0xffffffffu, ring.abort)) return false;
-        if (__any_sync(0xffffffffu, *const_cast<volatile int *>(&ring.slow))) i = 0;
-    }
-    ring.abort = 1;
-    return false;
-}
-
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float m;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
@@ -233,7 +222,7 @@ struct TcIssuer {
         go = tc_elect();
     }
     __device__ __forceinline__ void wait(uint64_t *b, uint32_t count) {
-        if (!tc_wait(sh.ring, b, count)) go = 0;
+        if (!warp_wait(sh.ring, b, count)) go = 0;
         tc_fence_after();
     }
     __device__ __forceinline__ void tile(uint32_t &stage) {
