@@ -399,21 +399,28 @@ __device__ __forceinline__ void paged_slow_row(const PagedArgs &a, const PagedIt
     __syncwarp();
 }
 
-// Zeros for the rows of no request: before the first, behind the last, of a refused one.
+// Zeros for the rows of no request, by block column x: those before the first and behind the
+// last.  Where a request does not fit, also the rows that it would have, and as its offsets may
+// then lie anywhere, no row that some request which fits has (the block looks each row up).
 template <int D, int MODE>
 __device__ __forceinline__ void paged_zero_rows(const PagedArgs &a) {
     const int64_t bytes = a.out_row * (MODE == PAGED_F32 ? 4 : 2);
-    auto zero = [&](int64_t r0, int64_t r1, int64_t step) {
-        for (int64_t r = r0; r < r1; r += step)
-            for (int64_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
-                *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + r * bytes + i) = make_uint4(0u, 0u, 0u, 0u);
+    auto any_request = [&](auto test) {
+        bool hit = false;
+        for (int b = threadIdx.x; b < a.requests; b += blockDim.x) hit |= test(paged_request(a, b));
+        return __syncthreads_or(hit) != 0;
     };
-    auto clamp = [&](int64_t r) { return r < 0 ? int64_t{0} : (r > a.rows ? a.rows : r); };
-    const int64_t r0 = a.requests ? clamp(a.starts[0]) : 0, r1 = a.requests ? clamp(a.starts[a.requests]) : 0;
-    zero(blockIdx.x, r0, gridDim.x);
-    zero(r1 + blockIdx.x, a.rows, gridDim.x);
-    for (int b = blockIdx.x; b < a.requests; b += gridDim.x)
-        if (paged_request(a, b).bad) zero(clamp(a.starts[b]), clamp(a.starts[b + 1]), 1);
+    const bool bad = any_request([](const PagedRequest &r) { return r.bad; });
+    const int64_t r0 = bad || !a.requests ? a.rows : a.starts[0], r1 = bad || !a.requests ? a.rows : a.starts[a.requests];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        if (row >= r0 && row < r1) {  // (the first row from r1 on that is this block's)
+            row += (r1 - 1 - row) / gridDim.x * gridDim.x;
+            continue;
+        }
+        if (bad && any_request([&](const PagedRequest &r) { return row >= r.row0 && row < r.row0 + int64_t{r.count}; })) continue;
+        for (int64_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+            *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + row * bytes + i) = make_uint4(0u, 0u, 0u, 0u);
+    }
 }
 
 // ------------------------------------------------------------------ tiles

@@ -466,13 +466,15 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * more new tokens (0: unknown); it saves the launch of kernels that no request
  * needs.  Rows of no request are left as they were, or set to zero when zero_fill.
  * A request whose lengths do not fit (rows, table_width, longest) is left out
- * (BD_FLAG_BAD_LENGTH); keys on a page outside the pool count as zeros
- * (BD_FLAG_BAD_PAGE); entries of pages that no token sees are not read.  What the
- * cache holds at keys that a row does not see never reaches it, not even as NaN:
- * a row whose own scores are all -infinity is not a number, as its softmax is;
- * a row with a value that is not finite is done again over its own keys, by one warp
- * and so slowly (0.3 to 0.9 us a key; the waits of its SM allow for it).  Strides as at bd_paged_store; caches are read
- * by TMA, so strides that a tensor map cannot hold are BD_ERR_ALIGNMENT too.
+ * (BD_FLAG_BAD_LENGTH), and its rows are rows of no request as far as no other has
+ * them; of requests whose rows overlap, those rows are undefined.  Keys on a page
+ * outside the pool count as zeros (BD_FLAG_BAD_PAGE); entries of pages that no token
+ * sees are not read.  What the cache holds at keys that a row does not see never
+ * reaches it, not even as NaN: a row with a value that is not finite is done again
+ * over its own keys, by one warp and so slowly (0.3 to 0.9 us a key; the waits of its
+ * SM allow for it).  A row whose own scores are all -infinity is not a number, as its
+ * softmax is.  Strides as at bd_paged_store; caches are read by TMA, so strides that
+ * a tensor map cannot hold are BD_ERR_ALIGNMENT too.
  * The workspace needs no clearing; calls that overlap on the GPU need their own.
  * Results do not depend on what else the GPU runs: partials are joined in order. */
 #define BD_F16 0

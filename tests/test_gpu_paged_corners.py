@@ -170,3 +170,39 @@ def test_a_request_that_is_not_finite_spoils_no_other(ops, row_type, count, keys
     flags.check()
     assert torch.equal(got[count:], want[count:])
     assert bool(torch.isnan(got[:count]).all()) and bool(torch.isfinite(want).all())
+
+
+# ------------------------------------------------------------------ lengths that do not fit
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("heads_each, context", [(1, 20), (1, 3000), (20, 300)])
+@pytest.mark.parametrize("starts", [[0, 1000, 8, 10], [0, 3, 1000, 8, 10, 5], [9, 20, 3, 5], [-4, 2, 1000, 6, 7], [4, 2, 10, 10, 3],
+                                    [0, 3, 3, 10, 6]])
+def test_refused_rows_do_not_touch_those_of_others(ops, row_type, heads_each, context, starts):
+    """Row offsets that do not ascend: each request that fits has its rows, whole items and
+    joined ones alike, and all rows that no such request claims are zero or stay."""
+    lib, rows, requests = submodule("_lib"), 10, len(starts) - 1
+    batch = Batch([(context, rows)] * requests, 2 * heads_each, 2, 64, 16, row_type, seed=51)
+    q = batch.q[:rows]
+    out = torch.full((rows, 2 * heads_each, 64), 7.0, dtype=row_type, device=DEV)
+    want, claims = torch.zeros_like(out), [0] * rows
+    for b in range(requests):
+        s, e = starts[b], starts[b + 1]
+        if 0 <= s <= e <= rows:
+            alone = ops.paged_attention(q[s:e], batch.k, batch.v, batch.table[b:b + 1], batch.context[:1], dev32([0, e - s]))
+            want[s:e] = alone
+            for r in range(s, e):
+                claims[r] += 1
+    assert max(claims) == 1
+    args = (q, batch.k, batch.v, batch.table, batch.context, dev32(starts))
+    free = torch.tensor(claims, device=DEV) == 0
+    u = HALF_STEP[row_type]
+    for _ in range(20):
+        flags = ops.Flags(DEV)
+        got, kept = ops.paged_attention(*args, flags=flags), ops.paged_attention(*args, out=out.clone(), flags=flags)
+        assert int(flags.tensor.item()) == lib.FLAG_BAD_LENGTH
+        assert not got[free].any() and bool((kept[free] == 7.0).all())
+        # another batch splits the work elsewhere: each side is within a rounding of P, O and the output
+        for x in (got, kept):
+            assert float((x[~free].double() - want[~free].double()).norm()) <= 4 * max(u, 2.0 ** -20) * float(want.double().norm())
