@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
             const int k = find_range(give_end, n, i);
             const int64_t at = (b0 + k) * a.table_ld + chunk[k].need + (i - (k ? give_end[k - 1] : 0));
             const int page = a.table[at];
+            checked_page(a, page);  // a bad one is reported by the step that gives it back too
             a.table[at] = -1;
             if (top + given + i < a.free_capacity)
                 a.free_list[top + given + i] = page;

@@ -446,7 +446,7 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * A request with lengths below zero or beyond table_width pages keeps its pages
  * and has no rows (BD_FLAG_BAD_LENGTH, as for more rows than `rows`, a top outside
  * [0, free_capacity] and a full stack); page ids outside [0, pool_pages) are not
- * used (BD_FLAG_BAD_PAGE).  Table entries of a request beyond the pages it owns are
+ * used (BD_FLAG_BAD_PAGE, also when they are given back to the stack).  Table entries of a request beyond the pages it owns are
  * not read.
  *
  * bd_paged_store: key and value row r (row and head strides in elements; 16-byte

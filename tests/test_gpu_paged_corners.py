@@ -206,3 +206,21 @@ def test_refused_rows_do_not_touch_those_of_others(ops, row_type, heads_each, co
         # another batch splits the work elsewhere: each side is within a rounding of P, O and the output
         for x in (got, kept):
             assert float((x[~free].double() - want[~free].double()).norm()) <= 4 * max(u, 2.0 ** -20) * float(want.double().norm())
+
+
+# ------------------------------------------------------------------ plan
+
+
+@pytest.mark.parametrize("page", [-1, 6, 2 ** 31 - 1, -2 ** 31])
+def test_plan_reports_a_bad_page_that_is_given_back(ops, page):
+    """By the step that gives it back, not only by one that would take it."""
+    lib, flags = submodule("_lib"), ops.Flags(DEV)
+    table, owned, free, top = dev32([[0, page, -1], [1, 2, -1]]), dev32([2, 2]), dev32([3, 4, 5, -9]), dev32([3])
+    ops.page_plan(dev32([0, 20]), dev32([0, 4]), table, owned, free, top, 16, 4, 6, flags=flags)
+    assert int(flags.tensor.item()) == lib.FLAG_BAD_LENGTH | lib.FLAG_BAD_PAGE  # the stack has room for one of the two
+    flags = ops.Flags(DEV)
+    table, owned, free, top = dev32([[0, page, -1], [1, 2, -1]]), dev32([2, 2]), dev32([3, 4, 5, -9, -9]), dev32([3])
+    ops.page_plan(dev32([0, 20]), dev32([0, 4]), table, owned, free, top, 16, 4, 6, flags=flags)
+    assert int(flags.tensor.item()) == lib.FLAG_BAD_PAGE
+    assert table.tolist() == [[-1, -1, -1], [1, 2, -1]] and owned.tolist() == [0, 2] and top.tolist() == [5]
+    assert free.tolist() == [3, 4, 5, 0, page]
