@@ -660,7 +660,9 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
     int32 ``[B]`` how many it has, ``free`` int32 a stack of free pages of which
     ``top`` int32 ``[1]`` are left.  Every request then owns exactly the pages that
     ``context + count`` positions need: missing ones are taken from the stack, those
-    beyond are given back (a finished request has both lengths 0).  ``table`` and
+    beyond are given back (a finished request has both lengths 0).  When the pages run
+    out, the first request that lacks too many and all later ones that lack any get none,
+    even if a later one's would be there.  ``table`` and
     ``free`` change in place, ``owned`` and ``top`` too unless ``owned_out`` and
     ``top_out`` are given.  Returns ``starts [B + 1]`` and, for ``rows`` rows,
     ``positions`` and ``slots`` (-1 behind the last request).  Without ``flags`` the

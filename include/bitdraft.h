@@ -440,7 +440,9 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * in order of request and entry, the missing entries, in the same order, are
  * S[|S| - 1], S[|S| - 2], ...  owned_out and top_out (which may be owned_in and
  * top_in) receive the new counts.  A request whose missing pages do not all fit
- * takes none (BD_FLAG_NO_PAGES).  starts[requests + 1]: exclusive sums of count;
+ * takes none (BD_FLAG_NO_PAGES), and neither does a later one: missing pages are
+ * counted in order of request, whether taken or not, so that a long request is not
+ * passed over for ever by short ones behind it.  starts[requests + 1]: exclusive sums of count;
  * positions / slots of each of `rows` rows: context[b] + t and page x page_size +
  * offset (slot -1 for a token without a page), -1 both behind the last request.
  * A request with lengths below zero or beyond table_width pages keeps its pages

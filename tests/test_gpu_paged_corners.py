@@ -224,3 +224,22 @@ def test_plan_reports_a_bad_page_that_is_given_back(ops, page):
     assert int(flags.tensor.item()) == lib.FLAG_BAD_PAGE
     assert table.tolist() == [[-1, -1, -1], [1, 2, -1]] and owned.tolist() == [0, 2] and top.tolist() == [5]
     assert free.tolist() == [3, 4, 5, 0, page]
+
+
+def test_plan_serves_no_request_behind_one_that_does_not_fit(ops):
+    """Five and one pages lacking, three free: neither is served, whichever has its pages there;
+    in the other order the small one is.  A request behind them that lacks none has its rows."""
+    lib = submodule("_lib")
+
+    def step(counts):
+        flags, table, owned = ops.Flags(DEV), torch.full((3, 6), -1, dtype=torch.int32, device=DEV), dev32([0, 0, 1])
+        table[2, 0] = 3
+        top = dev32([3])
+        plan = ops.page_plan(dev32([0, 0, 2]), dev32([*counts, 4]), table, owned, dev32([0, 1, 2, 9]), top, 16, sum(counts) + 4,
+                             10, flags=flags)
+        assert int(flags.tensor.item()) == lib.FLAG_NO_PAGES and plan.starts.tolist() == [0, counts[0], sum(counts), sum(counts) + 4]
+        return plan.slots.tolist(), owned.tolist(), top.tolist()
+
+    last = [3 * 16 + 2 + t for t in range(4)]
+    assert step((80, 16)) == ([-1] * 96 + last, [0, 0, 1], [3])
+    assert step((16, 80)) == ([2 * 16 + t for t in range(16)] + [-1] * 80 + last, [1, 0, 1], [2])
