@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
             else if (MODE == PAGED_BF16)
                 *reinterpret_cast<__nv_bfloat162 *>(static_cast<uint16_t *>(a.out) + at + i) = __floats2bfloat162_rn(o[i], o[i + 1]);
             else
-                *reinterpret_cast<__half2 *>(static_cast<uint16_t *>(a.out) + at + i) = __floats2half2_rn(o[i], o[i + 1]);
+                *reinterpret_cast<__half2 *>(static_cast<uint16_t *>(a.out) + at + i) =
+                    __floats2half2_rn(paged_bounded<MODE>(o[i]), paged_bounded<MODE>(o[i + 1]));
         }
     }
 }

@@ -50,6 +50,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// An output lies between the values that it weights, so fp16 ones are at most 65504, which the
+// roundings of the weights can pass by 2^-11.  (Rows that are not finite are done again.)
+template <int MODE>
+__device__ __forceinline__ float paged_bounded(float x) {
+    return MODE == PAGED_F16 ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
+}
+
 // row / groups for 0 <= row < 2^31: with 2^(s-1) < groups <= 2^s and the multiplier
 // m = ceil(2^(31+s) / groups) < 2^32, row m 2^-(31+s) exceeds row / groups by less than
 // row 2^-(31+s) < 1 / groups, so the floors agree.

@@ -386,7 +386,8 @@ __device__ __forceinline__ unsigned rows_stay(const PagedArgs &a, const PagedIte
                 if (F32)
                     *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at + n * 8 + 2 * t) = make_float2(x, y);
                 else
-                    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + at + n * 8 + 2 * t) = pack2<MODE>(x, y);
+                    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + at + n * 8 + 2 * t) =
+                        pack2<MODE>(paged_bounded<MODE>(x), paged_bounded<MODE>(y));
             }
             odd[r] = !(probe == 0.0f);
         }

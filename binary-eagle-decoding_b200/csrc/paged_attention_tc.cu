@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int k = 0; k < 8; ++k) {
                                 const float x = o[2 * k] * inv, y = o[2 * k + 1] * inv;
                                 probe += 0.0f * x + 0.0f * y;
-                                w[k] = tc_pack<MODE>(x, y);
+                                w[k] = tc_pack<MODE>(paged_bounded<MODE>(x), paged_bounded<MODE>(y));
                             }
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {

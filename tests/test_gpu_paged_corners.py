@@ -243,3 +243,22 @@ def test_plan_serves_no_request_behind_one_that_does_not_fit(ops):
     last = [3 * 16 + 2 + t for t in range(4)]
     assert step((80, 16)) == ([-1] * 96 + last, [0, 0, 1], [3])
     assert step((16, 80)) == ([2 * 16 + t for t in range(16)] + [-1] * 80 + last, [1, 0, 1], [2])
+
+
+# ------------------------------------------------------------------ the types' ends
+
+
+@pytest.mark.parametrize("requests, count, head_dim", [(3, 1, 128), (3, 200, 64), (40, 64, 128), (40, 64, 64), (160, 3, 128)])
+@pytest.mark.parametrize("value", [65504.0, -65504.0])
+def test_fp16_outputs_of_the_largest_values_are_finite(ops, requests, count, head_dim, value):
+    """An output lies between the values that it weights.  Every weight but the first key's is
+    one quarter x (1 + 1.2 x 2^-11), which fp16 rounds up by 0.8 x 2^-11: that must not carry
+    the output past the type's largest number."""
+    batch = Batch([(900, count)] * requests, 32, 8, head_dim, 16, torch.float16, seed=61)
+    batch.q = torch.zeros_like(batch.q)
+    batch.q[..., 0] = 1.0
+    batch.k.zero_()
+    batch.k[batch.table[:, 0].long(), 0, :, 0] = 1.0
+    batch.v.fill_(value)
+    got = batch.run(ops, scale=math.log(4.0 / (1 + 1.2 * 2.0 ** -11))).float()
+    assert bool(((got - value).abs() <= 65504.0 * 2.0 ** -10).all())  # (an infinity is not)
