@@ -349,7 +349,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // -------------------------------------------------- softmax: a thread to a row
         const int t = warp >> 2, wrow = (warp & 3) * 32, lrow = wrow + lane;
         const uint32_t s_at = tmem + t * 128 + (static_cast<uint32_t>(wrow) << 16), o_at = s_at + kO;
-        const float c = fmaxf(fabsf(a.scale_log2), 1e-37f);  // the scale's sign goes into Q
+        // the scale's sign goes into Q; not 0, as a masked -inf times it has to stay that (the smallest
+        // number there is, 2^-149, leaves every finite score at 0)
+        const float c = fmaxf(fabsf(a.scale_log2), 1.4e-45f);
         // 16-byte piece c of row r of 128 rows as the MMAs read them
         auto row_piece = [](uint8_t *rows, int r, int c) {
             return reinterpret_cast<uint4 *>(rows + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));

@@ -262,3 +262,18 @@ def test_fp16_outputs_of_the_largest_values_are_finite(ops, requests, count, hea
     batch.v.fill_(value)
     got = batch.run(ops, scale=math.log(4.0 / (1 + 1.2 * 2.0 ** -11))).float()
     assert bool(((got - value).abs() <= 65504.0 * 2.0 ** -10).all())  # (an infinity is not)
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("count, head_dim", [(1, 64), (40, 128)])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-40, 1e-38, -1e-38])
+def test_scales_near_zero(ops, row_type, count, head_dim, scale):
+    """Flat weights whatever the scores, or the scores times a scale below the normal numbers."""
+    batch = Batch([(90, count), (0, 3)], 4, 2, head_dim, 16, row_type, seed=62)
+    if row_type == torch.bfloat16:  # scores of about 1e36
+        batch.q, batch.k = batch.q * 1e18, batch.k.mul_(1e17)
+    want, *how = exact(batch, scale=scale)
+    err = (batch.run(ops, scale=scale).double() - want).abs()
+    # the scale itself is held to 2^-150, and 0 as 2^-149; the scores are below 1e38
+    lost = 2.0 ** -149 * 1e38 if row_type == torch.bfloat16 else 0.0
+    assert bool((err <= small_weights_bound(batch, want, *how) + 2.2 * lost * how[0]).all())
