@@ -30,6 +30,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <cmath>
 #include <mutex>
 
 namespace bd {
@@ -39,6 +40,7 @@ namespace bd {
 // tokens and 6 single tokens over 4096 keys, 8 kv heads: 149 us instead of 181, 14: 181 and
 // 202, 30: 251 and 246, 62: 386 and 326; 32 x 17 tokens over 2048 keys: 76 and 84).
 constexpr int kOneKernelPairs = 256;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Joins the partials of the items that lie across CTAs: CTA (x, y) those of the item
 // that CTA x (of the first kernel, then of the second) left open, a warp to a row, 8
@@ -220,7 +222,7 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
         p->heads > 65535 || p->rows > INT32_MAX / (p->heads / p->kv_heads) ||
         (p->head_dim != 64 && p->head_dim != 128) || !page_size_ok(p->page_size) ||
         !pool_ok(p->pool_pages, p->page_size) || !table_ok(p->table_width, p->page_size) ||
-        p->table_ld < p->table_width || p->window < 0 || p->longest < 0 || !(p->scale > -INFINITY && p->scale < INFINITY))
+        p->table_ld < p->table_width || p->window < 0 || p->longest < 0 || !std::isfinite(p->scale * kLog2e))
         return BD_ERR_INVALID;
     int mode;
     if (p->row_type == BD_F32 && p->cache_type == BD_F16)
@@ -261,7 +263,7 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     a.causal = p->causal != 0;
     a.window = p->window > INT32_MAX ? 0 : static_cast<int>(p->window);
     a.longest = p->longest ? p->longest : INT32_MAX;
-    a.scale_log2 = p->scale * 1.4426950408889634f;  // log2 e
+    a.scale_log2 = p->scale * kLog2e;
     a.out = p->out;
     a.out_row = static_cast<int64_t>(p->heads) * p->head_dim;
     a.zero_fill = p->zero_fill;

@@ -780,10 +780,15 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         window = 0
     elif window < 1:
         raise ValueError("window must be at least 1")
+    elif window > 0x7FFFFFFF:
+        window = 0  # positions are below it
     if longest is None:
         longest = rows
     elif longest < 1:
         raise ValueError("longest must be at least 1")
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < 2e38:  # (NaN too) times log2 e it is a fp32 number
+        raise ValueError("scale must be a number below 2e38 in size")
     index = q.get_device()
     _one_device(index, flags, k_cache, v_cache, table, context, starts)
     fresh = out is None
@@ -808,7 +813,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         q.data_ptr(), q_row, q_head, _ROW_TYPE[dtype], k_cache.data_ptr(), v_cache.data_ptr(), *k_strides[:3],
         *v_strides[:3], _CACHE_TYPE[k_cache.dtype], page_size, pages, table.data_ptr(), ld, table.shape[1],
         context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
-        min(longest, 0x7FFFFFFF), head_dim ** -0.5 if scale is None else scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
+        min(longest, 0x7FFFFFFF), scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
         flags.tensor.data_ptr())
     # fp16 and bf16 batches of more than 256 (request, kv head) pairs that may hold long requests
     both = (dtype is not torch.float32 and requests * kv_heads > 256

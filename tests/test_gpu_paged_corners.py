@@ -277,3 +277,10 @@ def test_scales_near_zero(ops, row_type, count, head_dim, scale):
     # the scale itself is held to 2^-150, and 0 as 2^-149; the scores are below 1e38
     lost = 2.0 ** -149 * 1e38 if row_type == torch.bfloat16 else 0.0
     assert bool((err <= small_weights_bound(batch, want, *how) + 2.2 * lost * how[0]).all())
+
+
+def test_windows_beyond_every_position_are_none(ops):
+    batch = Batch([(90, 20), (3, 1)], 4, 2, 64, 16, torch.float16, seed=63)
+    want = batch.run(ops)
+    for window in (110, 2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 80):
+        assert torch.equal(batch.run(ops, window=window), want)
