@@ -31,4 +31,17 @@ inline bool cache_strides(const int64_t *s, CacheStrides &out) {
     return s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && ((s[0] | s[1] | s[2]) & 7) == 0;
 }
 
+// The bytes [begin, end) that a strided tensor lies in.
+struct Span {
+    uintptr_t begin, end;
+    bool meets(const Span &o) const { return begin < o.end && o.begin < end; }
+};
+inline Span span_of(const void *p, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Span{at, at + static_cast<uintptr_t>(bytes)};
+}
+inline Span cache_span(const void *p, const CacheStrides &s, int64_t pages, int page_size, int heads, int head_dim) {
+    return span_of(p, 2 * ((pages - 1) * s.page + (page_size - 1) * s.slot + (heads - 1) * s.head + head_dim));
+}
+
 }  // namespace bd

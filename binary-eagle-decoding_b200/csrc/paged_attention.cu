@@ -268,6 +268,19 @@ extern "C" int bd_paged_attention(const bd_paged_attention_args *p, bd_stream_t 
     a.out_row = static_cast<int64_t>(p->heads) * p->head_dim;
     a.zero_fill = p->zero_fill;
     a.flags = p->flags;
+    // rows may be read after others are written
+    const int64_t each = mode == PAGED_F32 ? 4 : 2, q_rows = (p->rows - 1) * p->q_row, q_heads = (p->heads - 1) * p->q_head;
+    const int64_t q_first = std::min<int64_t>(q_rows, 0) + std::min<int64_t>(q_heads, 0);
+    const Span out = span_of(p->out, p->rows * a.out_row * each);
+    if (out.meets(span_of(static_cast<const char *>(p->q) + q_first * each,
+                          (std::max<int64_t>(q_rows, 0) + std::max<int64_t>(q_heads, 0) - q_first + p->head_dim) * each)) ||
+        out.meets(cache_span(p->k_cache, a.ks, a.pool, p->page_size, a.kv_heads, p->head_dim)) ||
+        out.meets(cache_span(p->v_cache, a.vs, a.pool, p->page_size, a.kv_heads, p->head_dim)) ||
+        (a.requests && (out.meets(span_of(p->table, 4 * ((a.requests - 1) * p->table_ld + p->table_width))) ||
+                        out.meets(span_of(p->context, 4 * int64_t{a.requests})) ||
+                        out.meets(span_of(p->starts, 4 * (int64_t{a.requests} + 1))))) ||
+        out.meets(span_of(p->workspace, static_cast<int64_t>(p->workspace_bytes))))
+        return BD_ERR_INVALID;
     const int64_t pairs = static_cast<int64_t>(a.requests) * a.kv_heads;
     a.item_rows = rows_item(p->head_dim, mode);
     a.split_rows = mode == PAGED_F32 ? INT_MAX : a.item_rows;

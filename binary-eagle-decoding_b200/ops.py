@@ -746,6 +746,12 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
 _Strides = _lib.c_int64 * 3
 
 
+def _span(t: Tensor) -> tuple[int, int]:
+    """The addresses [first, last) that a tensor lies in."""
+    reach = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + reach * t.element_size()
+
+
 def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, context: Tensor, starts: Tensor,
                     causal: bool = True, window: int | None = None, scale: float | None = None,
                     longest: int | None = None, out: Tensor | None = None, flags: Flags | None = None) -> Tensor:
@@ -758,7 +764,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
     than ``window`` positions away.  fp32 rows over an fp16 cache (the products keep
     fp32 precision), fp16 over fp16 or bf16 over bf16; head_dim 64 or 128.
     ``longest``: an upper bound of the requests' new tokens, when the caller knows
-    one.  Returns ``out`` (not a part of ``q``), whose rows of no request stay as they
+    one.  Returns ``out`` (over nothing that is read), whose rows of no request stay as they
     were; without ``out`` a new tensor in which they are zero."""
     pages, page_size, kv_heads, cache_dim = _cache_shape(k_cache, v_cache)
     shape, dtype = q.shape, q.dtype
@@ -798,6 +804,9 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         span = ((rows - 1) * q_row + (heads - 1) * q_head + head_dim) * q.element_size()
         if -out.nbytes < out.data_ptr() - q.data_ptr() < span:
             raise ValueError("out must not overlap q")
+        begin, end = out.data_ptr(), out.data_ptr() + out.nbytes
+        if any(begin < last and first < end for first, last in map(_span, (k_cache, v_cache, table, context, starts))):
+            raise ValueError("out must not overlap the caches, the table or the lengths")
     if index != _DEVICE():
         with torch.cuda.device(index):
             return paged_attention(q, k_cache, v_cache, table, context, starts, causal, window or None, scale, longest or 1,

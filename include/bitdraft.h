@@ -464,9 +464,10 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * stored first), s <= position when causal, |position - s| < window when window >
  * 0.  Query head h reads kv head h / (heads / kv_heads).  head_dim 64 or 128.
  * Types: fp32 rows over an fp16 cache at fp32 precision, fp16 over fp16, bf16 over
- * bf16; out [rows][heads][head_dim] has the type of q.  longest: no request has
- * more new tokens (0: unknown); it saves the launch of kernels that no request
- * needs.  Rows of no request are left as they were, or set to zero when zero_fill.
+ * bf16; out [rows][heads][head_dim] has the type of q and overlaps nothing that is
+ * read.  longest: no request has more new tokens (0: unknown); it saves the launch of
+ * kernels that no request needs.  Rows of no request are left as they were, or set to
+ * zero when zero_fill.
  * A request whose lengths do not fit (rows, table_width, longest) is left out
  * (BD_FLAG_BAD_LENGTH), and its rows are rows of no request as far as no other has
  * them; of requests whose rows overlap, those rows are undefined.  Keys on a page

@@ -284,3 +284,20 @@ def test_windows_beyond_every_position_are_none(ops):
     want = batch.run(ops)
     for window in (110, 2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 80):
         assert torch.equal(batch.run(ops, window=window), want)
+
+
+# ------------------------------------------------------------------ memory in common
+
+
+def test_attention_refuses_an_output_over_what_it_reads(ops):
+    batch = Batch([(30, 5), (7, 2)], 4, 2, 64, 16, torch.float16, seed=71)
+    for cache in (batch.k, batch.v):
+        out = cache.flatten()[64:64 + batch.q.numel()].view(batch.q.shape)
+        with pytest.raises(ValueError, match="must not overlap the caches"):
+            batch.run(ops, out=out)
+    # behind one another in a buffer is fine
+    buffer = torch.zeros(batch.k.numel() + batch.q.numel(), dtype=torch.float16, device=DEV)
+    buffer[:batch.k.numel()] = batch.k.flatten()
+    want = batch.run(ops)
+    batch.k = buffer[:batch.k.numel()].view(batch.k.shape)
+    assert torch.equal(batch.run(ops, out=buffer[batch.k.numel():].view(batch.q.shape)), want)

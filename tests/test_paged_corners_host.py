@@ -32,3 +32,20 @@ def test_attention_wrapper_refuses_scales_that_are_no_numbers_of_fp32(ops):
     for scale in (1e38, 0.0, -0.5, None):
         with pytest.raises(ValueError, match="CUDA tensors"):
             ops.paged_attention(**good, scale=scale)
+
+
+# byte sizes of the call of attention_args(): q and out 3 x 256 x 2, a cache 8 x 2048 x 2, the table 2 x 4 x 4
+Q, CACHE, OUT = 1536, 32768, 1536
+
+
+@pytest.mark.parametrize("name, place, size", [("q", 0x100000, Q), ("k_cache", 0x200000, CACHE), ("v_cache", 0x300000, CACHE),
+                                               ("table", 0x400000, 32), ("context", 0x500000, 8), ("starts", 0x600000, 12),
+                                               ("workspace", 0x10000000, 1 << 26)])
+@pytest.mark.parametrize("where", ["same", "last", "first"])
+def test_attention_entry_refuses_an_output_over_what_is_read(name, place, size, where):
+    lib = submodule("_lib")
+    places = dict(q=0x100000, k_cache=0x200000, v_cache=0x300000, table=0x400000, context=0x500000, starts=0x600000,
+                  workspace=0x10000000, workspace_bytes=1 << 26)
+    out = {"same": place, "last": place + (size - 1) // 16 * 16, "first": place - OUT + 16}[where]
+    args = attention_args(**places, out=out)
+    assert lib.load().bd_paged_attention(ctypes.byref(args), None) == 1
