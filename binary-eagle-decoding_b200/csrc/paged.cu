@@ -3,6 +3,7 @@
 // the device) and the store of new key and value rows into their slots.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "paged.cuh"
 
@@ -417,6 +418,20 @@ static int launch_store(const StoreArgs &a, bool bf16, cudaStream_t stream) {
                       stream, a);
 }
 
+// No two (page, slot, head) of a cache share an element: each stride is beyond all that the
+// smaller ones reach.
+static bool apart(const CacheStrides &s, int64_t pages, int page_size, int heads, int head_dim) {
+    std::pair<int64_t, int64_t> axes[3] = {{s.page, pages}, {s.slot, page_size}, {s.head, heads}};  // stride, size
+    std::sort(axes, axes + 3);
+    int64_t reach = head_dim;
+    for (auto &axis : axes) {
+        if (axis.second < 2) continue;
+        if (axis.first < reach) return false;
+        reach += (axis.second - 1) * axis.first;
+    }
+    return true;
+}
+
 extern "C" int bd_paged_store(const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
                               int row_type, const int32_t *slots, int64_t rows, int kv_heads, int head_dim,
                               int page_size, int64_t pool_pages, void *k_cache, const int64_t *k_strides,
@@ -450,6 +465,10 @@ extern "C" int bd_paged_store(const void *k, int64_t k_row, int64_t k_head, cons
     a.k_cache = static_cast<uint16_t *>(k_cache);
     a.v_cache = static_cast<uint16_t *>(v_cache);
     a.flags = flags;
+    // slots that share elements would be written in any order
+    if (!apart(a.ks, pool_pages, page_size, kv_heads, head_dim) || !apart(a.vs, pool_pages, page_size, kv_heads, head_dim) ||
+        span_of(k_cache, 2 * head_dim).meets(span_of(v_cache, 2 * head_dim)))
+        return BD_ERR_INVALID;
     const bool bf16 = cache_type == BD_BF16;
     if (row_type == BD_F32) return launch_store<float>(a, bf16, stream);
     if (row_type == BD_F16) return launch_store<__half>(a, bf16, stream);

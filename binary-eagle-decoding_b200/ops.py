@@ -714,7 +714,8 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
     """Key and value rows ``[rows, kv_heads, head_dim]`` (fp32, fp16 or bf16; views of a
     fused projection are fine) into slots ``page * page_size + offset`` of the caches
     ``[pages, page_size, kv_heads, head_dim]``, rounded to their type.  Rows with slot -1 are
-    skipped; a slot may appear once.  Raises (or flags) "F16 cache storage overflow"
+    skipped; a slot may appear once, and rows may lie in the caches only where no slot of
+    the call is.  Raises (or flags) "F16 cache storage overflow"
     when a stored value is not finite."""
     pages, page_size, kv_heads, head_dim = _cache_shape(k_cache, v_cache)
     shape, dtype = k.shape, k.dtype
@@ -736,9 +737,14 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
             return paged_store(k, v, slots, k_cache, v_cache, flags)
     own = flags is None
     flags = flags or Flags(k.device)
-    _lib.call("bd_paged_store", k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, _ROW_TYPE[dtype],
-              slots.data_ptr(), rows, kv_heads, head_dim, page_size, pages, k_cache.data_ptr(), _Strides(*k_strides),
-              v_cache.data_ptr(), _Strides(*v_strides), _CACHE_TYPE[k_cache.dtype], flags.tensor.data_ptr(), _raw_stream(index))
+    try:
+        _lib.call("bd_paged_store", k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, _ROW_TYPE[dtype],
+                  slots.data_ptr(), rows, kv_heads, head_dim, page_size, pages, k_cache.data_ptr(), _Strides(*k_strides),
+                  v_cache.data_ptr(), _Strides(*v_strides), _CACHE_TYPE[k_cache.dtype], flags.tensor.data_ptr(),
+                  _raw_stream(index))
+    except ValueError as error:
+        raise ValueError(f"{error}: head_dim must be a multiple of 8, and no two slots, heads or caches may share "
+                         "elements") from None
     if own:
         flags.check()
 

@@ -455,7 +455,9 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * aligned pieces) to slot slots[r] of the caches, rounded to their type; slots below
  * 0 are skipped, slots beyond the cache too (BD_FLAG_BAD_PAGE).  A stored value
  * that is not finite sets BD_FLAG_CACHE_OVERFLOW (model.py:100-101).  A slot given
- * twice in one call holds pieces of either row.  Strides: host int64 [3] (page,
+ * twice in one call holds pieces of either row.  The rows may lie in the caches (a
+ * page is copied that way) where no slot of the call is.  Caches in which two slots or
+ * heads share elements, or both caches do, are refused.  Strides: host int64 [3] (page,
  * slot, head), multiples of 8.
  *
  * bd_paged_attention: for token t of request b (row starts[b] + t, position

@@ -301,3 +301,24 @@ def test_attention_refuses_an_output_over_what_it_reads(ops):
     want = batch.run(ops)
     batch.k = buffer[:batch.k.numel()].view(batch.k.shape)
     assert torch.equal(batch.run(ops, out=buffer[batch.k.numel():].view(batch.q.shape)), want)
+
+
+def test_store_refuses_caches_that_share_elements(ops):
+    cache, rows, slots = torch.zeros((3, 16, 2, 64), dtype=torch.float16, device=DEV), torch.ones((5, 2, 64), device=DEV), dev32(range(5))
+    one = torch.zeros((1, 16, 2, 64), dtype=torch.float16, device=DEV)
+    for k, v in ((cache, cache), (one.expand(3, -1, -1, -1), cache), (cache, cache[:, :, :1].expand(-1, -1, 2, -1))):
+        with pytest.raises(ValueError, match="share elements"):
+            ops.paged_store(rows, rows, slots, k, v)
+    assert not cache.any() and not one.any()
+
+
+def test_a_page_is_copied_within_the_caches(ops):
+    """Rows that lie in the caches themselves, into slots of other pages."""
+    g = torch.Generator(device=DEV).manual_seed(72)
+    both = torch.randn((6, 16, 2, 3, 64), generator=g, device=DEV).half()
+    k, v = both[:, :, 0], both[:, :, 1]
+    want = both.clone()
+    want[5], want[2] = both[1], both[4]
+    for source, target in ((1, 5), (4, 2)):
+        ops.paged_store(k[source], v[source], torch.arange(target * 16, target * 16 + 16, dtype=torch.int32, device=DEV), k, v)
+    assert torch.equal(both, want)

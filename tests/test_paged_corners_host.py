@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from conftest import package, submodule
-from test_paged_host import attention_args, i32
+from test_paged_host import ADDR, attention_args, i32, store_args, strides
 
 
 @pytest.fixture(scope="module")
@@ -32,6 +32,20 @@ def test_attention_wrapper_refuses_scales_that_are_no_numbers_of_fp32(ops):
     for scale in (1e38, 0.0, -0.5, None):
         with pytest.raises(ValueError, match="CUDA tensors"):
             ops.paged_attention(**good, scale=scale)
+
+
+@pytest.mark.parametrize("k, v", [((2048, 128, 0), (2048, 128, 64)), ((2048, 128, 64), (2048, 0, 64)), ((0, 128, 64), (2048, 128, 64)),
+                                  ((2048, 64, 64), (2048, 128, 64)), ((2048, 128, 56), (2048, 128, 64)),
+                                  ((1920, 128, 64), (2048, 128, 64))])
+def test_store_entry_refuses_caches_whose_slots_share_elements(k, v):
+    """[8 pages][16 slots][2 heads][64 columns]; the second cache lies behind the first."""
+    args = store_args(k_strides=strides(*k), v_cache=ADDR + 2 * 8 * 2048, v_strides=strides(*v))
+    assert submodule("_lib").load().bd_paged_store(*args) == 1
+
+
+@pytest.mark.parametrize("offset", [0, 16, -16, 112, -112])
+def test_store_entry_refuses_caches_over_one_another(offset):
+    assert submodule("_lib").load().bd_paged_store(*store_args(k_cache=4096, v_cache=4096 + offset)) == 1
 
 
 # byte sizes of the call of attention_args(): q and out 3 x 256 x 2, a cache 8 x 2048 x 2, the table 2 x 4 x 4
