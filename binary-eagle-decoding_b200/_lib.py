@@ -253,10 +253,11 @@ launches = 0
 _SIZES: dict[tuple, int] = {}
 
 
-def size(name: str, *args) -> int:
+def size(name: str, *args, device: int | None = None) -> int:
     """A size query of the library (``bd_*_bytes``, ``*_partials``, ``*_ld``, ...), memoised:
-    each is a pure function of its integer arguments within a process."""
-    key = (name,) + args
+    each is a pure function of its integer arguments within a process, and of the number
+    of SMs of the current CUDA device where ``device``, its index, is given."""
+    key = (name, device) + args
     hit = _SIZES.get(key)
     if hit is None:
         hit = _SIZES[key] = int(getattr(load(), name)(*args))

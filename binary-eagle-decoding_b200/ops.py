@@ -819,7 +819,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
                                    out, flags)
     if fresh:
         out = q.new_empty(shape)
-    nbytes = _lib.size("bd_paged_attention_workspace_bytes", head_dim)
+    nbytes = _lib.size("bd_paged_attention_workspace_bytes", head_dim, device=index)
     # a buffer of this call: concurrent streams and captured graphs share none
     ws = context.new_empty(nbytes // 4)
     own = flags is None

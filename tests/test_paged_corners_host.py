@@ -63,3 +63,27 @@ def test_attention_entry_refuses_an_output_over_what_is_read(name, place, size, 
     out = {"same": place, "last": place + (size - 1) // 16 * 16, "first": place - OUT + 16}[where]
     args = attention_args(**places, out=out)
     assert lib.load().bd_paged_attention(ctypes.byref(args), None) == 1
+
+
+def test_sizes_that_depend_on_the_device_are_kept_by_device(monkeypatch):
+    """Two GPUs of different SM counts in one process: each has the workspace of its own."""
+    lib = submodule("_lib")
+
+    class Fake:
+        sms = 0
+
+        def bd_paged_attention_workspace_bytes(self, head_dim):
+            return head_dim * self.sms
+
+    fake = Fake()
+    monkeypatch.setattr(lib, "load", lambda: fake)
+    monkeypatch.setattr(lib, "_SIZES", {})
+    for device, sms in ((0, 100), (1, 148), (0, 100), (1, 148)):
+        fake.sms = sms
+        assert lib.size("bd_paged_attention_workspace_bytes", 128, device=device) == 128 * sms
+
+
+def test_attention_asks_for_the_workspace_of_its_device(ops):
+    import inspect
+
+    assert 'size("bd_paged_attention_workspace_bytes", head_dim, device=index)' in inspect.getsource(ops.paged_attention)
