@@ -707,7 +707,10 @@ def page_plan(context: Tensor, count: Tensor, table: Tensor, owned: Tensor, free
     return PagePlan(starts, positions, slots)
 
 
+# for the launch accounting: the CUDA sources' own constants
 _PLAN_ROWS = 4096  # rows that the plan's one CTA fills itself
+_ONE_KERNEL_PAIRS = 256
+_FEW_ROWS = {64: 32, 128: 16}  # rows per kv head of the mma.sync kernel, by head_dim
 
 
 def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor, flags: Flags | None = None) -> None:
@@ -741,7 +744,7 @@ def paged_store(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: T
         _lib.call("bd_paged_store", k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, _ROW_TYPE[dtype],
                   slots.data_ptr(), rows, kv_heads, head_dim, page_size, pages, k_cache.data_ptr(), _Strides(*k_strides),
                   v_cache.data_ptr(), _Strides(*v_strides), _CACHE_TYPE[k_cache.dtype], flags.tensor.data_ptr(),
-                  _raw_stream(index))
+                  _raw_stream(index), kernels=1 if rows else 0)
     except ValueError as error:
         raise ValueError(f"{error}: head_dim must be a multiple of 8, and no two slots, heads or caches may share "
                          "elements") from None
@@ -830,10 +833,10 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
         context.data_ptr(), starts.data_ptr(), requests, rows, heads, kv_heads, head_dim, causal, window,
         min(longest, 0x7FFFFFFF), scale, out.data_ptr(), fresh, ws.data_ptr(), nbytes,
         flags.tensor.data_ptr())
-    # fp16 and bf16 batches of more than 256 (request, kv head) pairs that may hold long requests
-    both = (dtype is not torch.float32 and requests * kv_heads > 256
-            and min(longest, rows) * (heads // kv_heads) > (16 if head_dim == 128 else 32))
-    _lib.call("bd_paged_attention", args, _raw_stream(index), kernels=2 + both)
+    # 16-bit batches of many (request, kv head) pairs that may hold long requests take both kernels
+    both = (dtype is not torch.float32 and requests * kv_heads > _ONE_KERNEL_PAIRS
+            and min(longest, rows) * (heads // kv_heads) > _FEW_ROWS[head_dim])
+    _lib.call("bd_paged_attention", args, _raw_stream(index), kernels=2 + both if rows else 0)
     if own:
         flags.check()
     return out

@@ -3,6 +3,7 @@ types' limits, values that are not finite, lengths that do not fit (needs a B200
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -322,3 +323,38 @@ def test_a_page_is_copied_within_the_caches(ops):
     for source, target in ((1, 5), (4, 2)):
         ops.paged_store(k[source], v[source], torch.arange(target * 16, target * 16 + 16, dtype=torch.int32, device=DEV), k, v)
     assert torch.equal(both, want)
+
+
+# ------------------------------------------------------------------ launches
+
+
+def test_launches_are_counted_as_made(ops):
+    """Against the nodes of a captured graph; none for calls without rows."""
+    lib, runtime = submodule("_lib"), ctypes.CDLL("libcudart.so.12")
+    flags, pages, no_rows = ops.Flags(DEV), dev32([[0, 1, 2, 3]]), dev32([0, 0])
+
+    def counted(call):
+        call()
+        torch.cuda.synchronize()
+        graph, nodes = torch.cuda.CUDAGraph(keep_graph=True), ctypes.c_size_t()
+        before = lib.launches
+        with torch.cuda.graph(graph):
+            call()
+        assert runtime.cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+        made = nodes.value
+        assert made == lib.launches - before
+        return made
+
+    for row_type, lengths, kv_heads, want in ((torch.float32, [(30, 80)] * 70, 4, 2), (torch.float16, [(30, 3)] * 70, 4, 2),
+                                              (torch.float16, [(30, 80)] * 64, 4, 2), (torch.float16, [(30, 80)] * 65, 4, 3)):
+        batch = Batch(lengths, 8, kv_heads, 64, 16, row_type, seed=81)
+        assert counted(lambda: batch.run(ops, longest=lengths[0][1], flags=flags)) == want
+    none = batch.q[:0]
+    assert counted(lambda: ops.paged_attention(none, batch.k, batch.v, batch.table[:1], batch.context[:1], no_rows, flags=flags)) == 0
+    k = torch.zeros((3, 4, 64), device=DEV)
+    slots = dev32([0, 1, 2])
+    assert counted(lambda: ops.paged_store(k, k, slots, batch.k, batch.v, flags=flags)) == 1
+    assert counted(lambda: ops.paged_store(k[:0], k[:0], slots[:0], batch.k, batch.v, flags=flags)) == 0
+    one, zero, free, top = dev32([1]), dev32([0]), dev32([0, 1]), dev32([2])
+    for rows, want in ((0, 1), (4096, 1), (4097, 2)):
+        assert counted(lambda: ops.page_plan(one, zero, pages, one, free, top, 16, rows, 4, flags=flags)) == want

@@ -87,3 +87,15 @@ def test_attention_asks_for_the_workspace_of_its_device(ops):
     import inspect
 
     assert 'size("bd_paged_attention_workspace_bytes", head_dim, device=index)' in inspect.getsource(ops.paged_attention)
+
+
+def test_launch_accounting_has_the_sources_constants(ops):
+    import re
+    from pathlib import Path
+
+    csrc = Path(submodule("_lib").__file__).parent / "csrc"
+    plan, attention, shared = ((csrc / f"{n}").read_text() for n in ("paged.cu", "paged_attention.cu", "paged_attention.cuh"))
+    assert int(re.search(r"kPlanRows = (\d+);", plan)[1]) == ops._PLAN_ROWS
+    assert int(re.search(r"kOneKernelPairs = (\d+);", attention)[1]) == ops._ONE_KERNEL_PAIRS
+    narrow, wide = re.search(r"head_dim == 64 \? (\d+) : (\d+)\);", shared).groups()
+    assert {64: int(narrow), 128: int(wide)} == ops._FEW_ROWS
