@@ -11,16 +11,17 @@
 // hide under the 2800 cycles that a tile takes to come from HBM: 64 requests over 1024 to
 // 8192 keys (1.09 GB) take 171 us = 6.4 TB/s, one over 131072 keys 94 us = 5.7 TB/s.
 // fp32 rows do twice the MMAs and are bound by these and by the chain through a tile from
-// 64 rows on: 24 draft blocks in a window of 4096 take 172 us, 53 % of the MMA pipe.
+// 64 rows on: 24 draft blocks in a window of 4096 take 169 us, 54 % of the MMA pipe.
 #include "paged_attention.cuh"
 
 namespace bd {
 
 constexpr int kRowsWarps = 8;
 constexpr int kPlane = 64;  // rows of a plane of Q in shared memory
-// A stay's Q, joining and output, in units; the tiles of fp32 rows of 128 columns take longer
-// (64 ragged tokens: 197 us with 1, 185 with 2, 184 with 4, of 64 columns 127, 119 and 112; 24
-// draft blocks 164, 157 and 160).
+// A stay's Q, joining and output, in units.  Other batches than those above: 64 tokens over 291,000
+// keys (1.19 GB) take 199 us with 1, 189 with 2, 184 with 4, of 64 columns 123, 118 and 113; 24
+// draft blocks over 1024 to 8192 keys in a window of 4096 take 170, 163 and 162, over 4096
+// keys each 184, 180 and 180, where 2 and 4 do not differ.
 template <int D, int MODE>
 constexpr int rows_extra() {
     return MODE == PAGED_F32 && D == 128 ? 2 : 4;

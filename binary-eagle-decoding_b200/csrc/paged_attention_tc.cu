@@ -23,10 +23,10 @@
 // and O += P V (P in TMEM, V as it lies, its rows being the reduction).
 //
 // What bounds it: in the steady state the softmax's chain of a step (two 2048-token chunks
-// over 8192 more keys: 575 us = 1075 TFLOP/s; with the softmax left out it would be 1350),
+// over 8192 more keys: 575 us = 1075 TFLOP/s, at the GPU's power limit 650; with the softmax left out it would be 1350),
 // and some 10,000 cycles a stay for Q, the first products and the output (over 4096 more
 // keys 340 us = 1010 TFLOP/s, ragged chunks of 64 columns in a window of 1000 keys 51 us).
-// Verification (32 requests of 68 rows over 0.5 to 4 K keys) takes 64 us = 4.4 TB/s.
+// Verification (32 requests of 68 rows over 0.5 to 4 K keys) takes 62 us = 4.5 TB/s.
 //
 // Every wait is bounded; one that runs out sets BD_FLAG_TIMEOUT and turns the waits
 // that follow into passes, so that all roles walk to their end.

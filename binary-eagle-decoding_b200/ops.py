@@ -771,7 +771,9 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
     (``paged_store``).  A token sees the request's keys at or before its position, or all
     of them when not ``causal`` (a draft block), and with ``window`` only those less
     than ``window`` positions away.  fp32 rows over an fp16 cache (the products keep
-    fp32 precision), fp16 over fp16 or bf16 over bf16; head_dim 64 or 128.
+    fp32 precision), fp16 over fp16 or bf16 over bf16 (the softmax weights are rounded
+    to that type, which adds about 0.4 of the output's rounding); head_dim 64 or 128.
+    A row whose own scores are all -infinity, or one of them NaN, is not a number.
     ``longest``: an upper bound of the requests' new tokens, when the caller knows
     one.  Returns ``out`` (over nothing that is read), whose rows of no request stay as they
     were; without ``out`` a new tensor in which they are zero."""

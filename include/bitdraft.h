@@ -442,14 +442,14 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * top_in) receive the new counts.  A request whose missing pages do not all fit
  * takes none (BD_FLAG_NO_PAGES), and neither does a later one: missing pages are
  * counted in order of request, whether taken or not, so that a long request is not
- * passed over for ever by short ones behind it.  starts[requests + 1]: exclusive sums of count;
- * positions / slots of each of `rows` rows: context[b] + t and page x page_size +
- * offset (slot -1 for a token without a page), -1 both behind the last request.
- * A request with lengths below zero or beyond table_width pages keeps its pages
- * and has no rows (BD_FLAG_BAD_LENGTH, as for more rows than `rows`, a top outside
- * [0, free_capacity] and a full stack); page ids outside [0, pool_pages) are not
- * used (BD_FLAG_BAD_PAGE, also when they are given back to the stack).  Table entries of a request beyond the pages it owns are
- * not read.
+ * passed over for ever by short ones behind it.  starts[requests + 1]: exclusive sums
+ * of count; positions / slots of each of `rows` rows: context[b] + t and page x
+ * page_size + offset (slot -1 for a token without a page), -1 both behind the last
+ * request.  A request with lengths below zero or beyond table_width pages keeps its
+ * pages and has no rows (BD_FLAG_BAD_LENGTH, as for more rows than `rows`, a top
+ * outside [0, free_capacity] and a full stack); page ids outside [0, pool_pages) are
+ * not used (BD_FLAG_BAD_PAGE, also when they are given back to the stack).  Table
+ * entries of a request beyond the pages it owns are not read.
  *
  * bd_paged_store: key and value row r (row and head strides in elements; 16-byte
  * aligned pieces) to slot slots[r] of the caches, rounded to their type; slots below
@@ -465,11 +465,13 @@ int bd_attention_decode(const float *q, const uint16_t *k_cache, const uint16_t 
  * context[b] + count (count = starts[b + 1] - starts[b]; the new tokens' own keys are
  * stored first), s <= position when causal, |position - s| < window when window >
  * 0.  Query head h reads kv head h / (heads / kv_heads).  head_dim 64 or 128.
- * Types: fp32 rows over an fp16 cache at fp32 precision, fp16 over fp16, bf16 over
- * bf16; out [rows][heads][head_dim] has the type of q and overlaps nothing that is
- * read.  longest: no request has more new tokens (0: unknown); it saves the launch of
- * kernels that no request needs.  Rows of no request are left as they were, or set to
- * zero when zero_fill.
+ * Types: fp32 rows over an fp16 cache at fp32 precision; fp16 over fp16, bf16 over
+ * bf16, whose softmax weights are rounded to that type (relative 2^-11 and 2^-8 at
+ * most, fp16 ones under 2^-25 of the row's largest to 2^-36 of it).  out
+ * [rows][heads][head_dim] has the type of q and overlaps nothing that is read.
+ * longest: no request has more new tokens (0: unknown); it saves the launch of kernels
+ * that no request needs.  Rows of no request are left as they were, or set to zero
+ * when zero_fill.
  * A request whose lengths do not fit (rows, table_width, longest) is left out
  * (BD_FLAG_BAD_LENGTH), and its rows are rows of no request as far as no other has
  * them; of requests whose rows overlap, those rows are undefined.  Keys on a page
