@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from conftest import package, submodule
-from test_gpu_paged import DEV, HALF_STEP, TYPES, Batch, dev32
+from test_gpu_paged import DEV, HALF_STEP, TYPES, Batch, check, dev32
 
 pytestmark = pytest.mark.gpu
 
@@ -358,3 +358,76 @@ def test_launches_are_counted_as_made(ops):
     one, zero, free, top = dev32([1]), dev32([0]), dev32([0, 1]), dev32([2])
     for rows, want in ((0, 1), (4096, 1), (4097, 2)):
         assert counted(lambda: ops.page_plan(one, zero, pages, one, free, top, 16, rows, 4, flags=flags)) == want
+
+
+# ------------------------------------------------------------------ long rows, captured steps
+
+
+@pytest.mark.parametrize("row_type", TYPES)
+@pytest.mark.parametrize("count, head_dim", [(1, 128), (20, 64), (40, 128), (300, 128)])
+@pytest.mark.parametrize("rate", [0.001, 0.005, -0.005, 0.03])
+def test_scores_that_grow_along_the_keys(ops, row_type, count, head_dim, rate):
+    """Each tile raises the running maximum, by less and by more than what is left unscaled."""
+    if row_type == torch.float32 and rate == 0.03:
+        rate = 0.01  # scores of 20, whose fp32 rounding the norm's limit allows for
+    lengths = [(1700, count), (900, 2)]
+    batch = Batch(lengths, 4, 2, head_dim, 16, row_type, seed=91)
+    q = batch.q.clone()
+    q[..., 0] = 4.0
+    batch.q = q
+    for b, (context, n) in enumerate(lengths):
+        at = torch.arange(context + n, device=DEV)
+        batch.k[batch.table[b, at // 16].long(), at % 16, :, 0] = (at * rate * head_dim ** 0.5 / 4)[:, None].to(batch.k.dtype)
+    check(ops, batch)
+    check(ops, batch, causal=False, window=500)
+
+
+def test_a_captured_step_replays_with_new_lengths(ops):
+    """Plan, store and attention in one graph over buffers of fixed size, replayed while requests
+    grow, pause and finish, against the same step made eagerly on copies."""
+    heads, kv_heads, d, page, pool, rows, requests = 8, 2, 64, 16, 64, 40, 4
+    g = torch.Generator(device=DEV).manual_seed(92)
+    flags = ops.Flags(DEV)
+
+    def state():
+        return dict(table=torch.full((requests, 16), -1, dtype=torch.int32, device=DEV), owned=dev32([0] * requests),
+                    free=torch.arange(pool, dtype=torch.int32, device=DEV), top=dev32([pool]),
+                    k=torch.zeros((pool, page, kv_heads, d), dtype=torch.float16, device=DEV),
+                    v=torch.zeros((pool, page, kv_heads, d), dtype=torch.float16, device=DEV))
+
+    context, count = dev32([0] * requests), dev32([0] * requests)
+    q = torch.zeros((rows, heads, d), dtype=torch.float16, device=DEV)
+    kv = torch.zeros((rows, 2 * kv_heads, d), dtype=torch.float16, device=DEV)
+
+    def step(s):
+        plan = ops.page_plan(context, count, s["table"], s["owned"], s["free"], s["top"], page, rows, pool, flags=flags)
+        ops.paged_store(kv[:, :kv_heads], kv[:, kv_heads:], plan.slots, s["k"], s["v"], flags=flags)
+        out = ops.paged_attention(q, s["k"], s["v"], s["table"], context, plan.starts, flags=flags)
+        return plan, out
+
+    mine, other = state(), state()
+    step(other)  # (no rows yet)
+    stream = torch.cuda.Stream(DEV)
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        plan, out = step(mine)
+    lengths = [0] * requests
+    for counts, finished in (([20, 1, 0, 19], ()), ([1, 1, 30, 8], ()), ([16, 0, 1, 1], (1,)), ([5, 33, 1, 1], ()),
+                             ([0, 1, 38, 1], (0, 3)), ([1, 1, 1, 1], ()), ([10, 10, 10, 10], ())):
+        for b in finished:
+            lengths[b] = 0
+        context.copy_(dev32(lengths))
+        count.copy_(dev32(counts))
+        q.copy_(torch.randn(q.shape, generator=g, device=DEV))
+        kv.copy_(torch.randn(kv.shape, generator=g, device=DEV))
+        torch.cuda.synchronize()
+        graph.replay()
+        want_plan, want = step(other)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(plan, want_plan)) and torch.equal(out, want)
+        assert all(torch.equal(mine[name], other[name]) for name in mine)
+        assert not out[sum(counts):].any()
+        lengths = [a + b for a, b in zip(lengths, counts)]
+        assert int(mine["top"]) == pool - sum(-(-n // page) for n in lengths)
+    flags.check()
